@@ -11,7 +11,12 @@ from .layer import (Activation, Convolution, ESigmoid, GeLU, HardTanH, Layer, Li
                     ReLU, Sigmoid, TanH)
 from .networks import DKPPCN, FullPCN, SimplePCN  # noqa: F401
 from .conv import SimpleConvolutionalPCN  # noqa: F401
+from .operators import (PackedActivations, ResidualNormGradients, VocabGradients,  # noqa: F401
+                        activate_and_pack, packed_activation_backward, residual_norm,
+                        residual_norm_backward, vocab_cross_entropy, vocab_cross_entropy_backward)
 from ._lib import DeepityError  # noqa: F401
 
 __all__ = ["DKPPCN", "FullPCN", "SimplePCN", "SimpleConvolutionalPCN", "Convolution", "Linear", "Sigmoid", "TanH", "ReLU", "GeLU",
-           "ESigmoid", "HardTanH", "DeepityError"]
+           "ESigmoid", "HardTanH", "DeepityError", "PackedActivations", "ResidualNormGradients", "VocabGradients",
+           "activate_and_pack", "packed_activation_backward", "residual_norm", "residual_norm_backward",
+           "vocab_cross_entropy", "vocab_cross_entropy_backward"]

@@ -15,6 +15,37 @@ LIB_PATH = os.path.join(_PKG, "libdeepity_b200.so")
 c_f32p = ctypes.POINTER(ctypes.c_float)
 _i, _f, _vp, _cp, _i64 = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int64
 
+_p, _sz, _i32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32
+
+
+class VocabCe(ctypes.Structure):
+    """dpc_vocab_ce"""
+    _fields_ = [("rows", _i64), ("width", _i64), ("vocab", _i64),
+                ("hidden_stride", _i64), ("weight_stride", _i64),
+                ("type", _i32), ("scale", _f), ("ignore_index", _i64),
+                ("hidden", _p), ("weight", _p), ("bias", _p), ("targets", _p), ("loss", _p), ("lse", _p),
+                ("grad_loss", _p), ("grad_stride", _i64),
+                ("d_hidden", _p), ("d_weight", _p), ("d_hidden_stride", _i64), ("d_weight_stride", _i64),
+                ("d_bias", _p), ("workspace", _p), ("workspace_bytes", _sz)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """dpc_residual_norm"""
+    _fields_ = [("rows", _i64), ("width", _i64), ("groups", _i64),
+                ("type", _i32), ("norm", _i32), ("post_norm", _i32),
+                ("stream_scale", _f), ("branch_scale", _f), ("eps", _f),
+                ("stream", _p), ("branch", _p), ("gate", _p), ("post_weight", _p), ("post_bias", _p),
+                ("pre_weight", _p), ("pre_bias", _p),
+                ("stream_stride", _i64), ("branch_stride", _i64), ("gate_stride", _i64),
+                ("new_stream", _p), ("normed", _p), ("new_stream_stride", _i64), ("normed_stride", _i64),
+                ("stats", _p),
+                ("d_normed", _p), ("d_new_stream", _p), ("d_normed_stride", _i64), ("d_new_stream_stride", _i64),
+                ("d_stream", _p), ("d_branch", _p), ("d_gate", _p),
+                ("d_stream_stride", _i64), ("d_branch_stride", _i64), ("d_gate_stride", _i64),
+                ("d_post_weight", _p), ("d_post_bias", _p), ("d_pre_weight", _p), ("d_pre_bias", _p),
+                ("workspace", _p), ("workspace_bytes", _sz)]
+
+
 # name -> (restype, argtypes); every symbol include/deepity_b200.h declares.
 SIGNATURES = {
     "dpc_last_error": (_cp, []),
@@ -136,6 +167,14 @@ SIGNATURES = {
     "dpcn_conv_context": (_vp, [_vp]),
     "dpcn_conv_plan": (_vp, [_vp]),
     "dpcn_conv_launch_count": (_i64, [_vp]),
+    "dpc_vocab_ce_workspace": (_i, [ctypes.POINTER(VocabCe), _i, ctypes.POINTER(_sz)]),
+    "dpc_vocab_ce_forward": (_i, [_vp, ctypes.POINTER(VocabCe)]),
+    "dpc_vocab_ce_backward": (_i, [_vp, ctypes.POINTER(VocabCe)]),
+    "dpc_residual_norm_forward": (_i, [_vp, ctypes.POINTER(ResidualNorm)]),
+    "dpc_residual_norm_workspace": (_i, [ctypes.POINTER(ResidualNorm), ctypes.POINTER(_sz)]),
+    "dpc_residual_norm_backward": (_i, [_vp, ctypes.POINTER(ResidualNorm)]),
+    "dpc_activate_and_pack": (_i, [_vp, _i, _i, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "dpc_packed_activation_backward": (_i, [_vp, _i, _i, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64]),
 }
 
 _lib = None

@@ -1,0 +1,114 @@
+// Shared by the operators that work on a caller's stream (dpc_vocab.cu, dpc_norm.cu, dpc_pack.cu):
+// the two tensor types, and the guard and checks of their C entries.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <exception>
+#include <string>
+
+#include "dpc_internal.h"
+
+namespace dpc
+{
+namespace ops
+{
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v)
+{
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v)
+{
+  return __float2bfloat16_rn(v);
+}
+
+// Eight values to and from bf16 in 16 bytes.
+__device__ __forceinline__ uint4 pack8(const float* v)
+{
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+  {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    r[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void unpack8(const uint4& p, float* v)
+{
+  const uint32_t r[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+  {
+    v[2 * i] = __uint_as_float(r[i] << 16);
+    v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+  }
+}
+
+// Eight neighbours in one or two 16-byte accesses.
+__device__ __forceinline__ void load8w(const float* p, float* v)
+{
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load8w(const __nv_bfloat16* p, float* v)
+{
+  unpack8(__ldg(reinterpret_cast<const uint4*>(p)), v);
+}
+__device__ __forceinline__ void store8w(float* p, const float* v)
+{
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8w(__nv_bfloat16* p, const float* v) { *reinterpret_cast<uint4*>(p) = pack8(v); }
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's tensor-map encoder, NULL where there is none.
+inline EncodeTiledFn encode_fn()
+{
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+  }();
+  return fn;
+}
+
+inline int launched(const char* what)
+{
+  const cudaError_t err = cudaPeekAtLastError();
+  return err == cudaSuccess ? (int)DPC_OK : cuda_fail(cudaGetLastError(), what);
+}
+
+// No C++ exception leaves a C entry.
+template <typename F>
+int guarded(const char* who, F f)
+{
+  try
+  {
+    return f();
+  }
+  catch (const std::exception& e)
+  {
+    return fail(DPC_ERR_CUDA, std::string(who) + ": " + e.what());
+  }
+  catch (...)
+  {
+    return fail(DPC_ERR_CUDA, std::string(who) + ": unknown exception");
+  }
+}
+} // namespace ops
+} // namespace dpc

@@ -1,0 +1,994 @@
+// Softmax cross entropy over a large vocabulary, with its gradient, in pieces of the vocabulary:
+// the [rows, vocab] logits are never kept.
+//
+//   l[n,v] = scale * sum_k hidden[n,k] weight[v,k] + bias[v]
+//   lse[n] = log sum_v exp l[n,v]          loss[n] = lse[n] - l[n, target[n]]
+//   s[n,v] = scale * g[n] * (exp(l[n,v] - lse[n]) - [v == target[n]])         g = dL/dloss
+//   d_hidden = s weight      d_weight = s^T hidden      d_bias = sum_n s / scale
+//
+// Forward: one product whose epilogue keeps, of every 128 columns, the maximum and the sum of the
+// exponentials of a row (8 bytes instead of 128 logits), then a kernel that joins them.  Backward, for
+// a piece of the vocabulary at a time: the product again with an epilogue that writes s, then
+// d_hidden += s weight and d_weight = s^T hidden.  The piece bounds the memory (s of one piece) and the
+// recomputed product is a quarter of the arithmetic; keeping the logits of 8192 rows x 128000 words in 32
+// bits instead would be 4.2 GB.
+//
+// One persistent kernel does all four products: 256 x 256 tiles on CTA pairs (cta_group::2), 64-deep
+// stages filled by TMA, accumulators double-buffered in tensor memory so that the epilogue warps work
+// on a tile while the next one is multiplied.  A row of the vocabulary or a batch of any length is a tile
+// whose outside TMA fills with zeros.
+//
+// 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low) in the six products
+// whose terms reach 2^-24, smallest first; s is held in as many planes.  For bf16 tensors s is rounded to
+// bf16 (half a step, 2^-9, of each of its values): the tensor cores take no wider operand beside bf16
+// weights, and the sums over it are in 32 bits and are rounded to bf16 themselves.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "dpc_internal.h"
+#include "dpc_operators.cuh"
+#include "dpc_tcgen05.cuh"
+
+namespace
+{
+using namespace dpc::ptx;
+using namespace dpc::ops;
+
+constexpr int kTile = 256;       // rows and columns of a pair's tile
+constexpr int kRows = 128;       // rows of A, and of B, that one CTA holds
+constexpr int kDepth = 64;       // contraction depth of a stage: 128 bytes, one swizzle row
+constexpr int kStages = 6;
+constexpr int kOperandBytes = kRows * kDepth * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+constexpr int kTmemColumns = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Bytes of slope, and of weight planes, that a piece of the vocabulary may take.
+constexpr size_t kPieceBytes = (size_t)256 << 20;
+
+enum Epilogue
+{
+  EPI_LSE,   // maximum and sum of exponentials of 128 columns of a row
+  EPI_SLOPE, // s of the piece, in bf16 planes
+  EPI_SUM,   // 32-bit sums, added to what earlier pieces left
+  EPI_OUT    // the product itself, in the type of the tensors
+};
+
+struct GemmParams
+{
+  int64_t tiles_m, tiles_n, group_m, items; // items = splits * tiles_m * tiles_n
+  int splits, kblocks, passes;
+  uint32_t plane_a, plane_b; // plane of a pass, 4 bits each
+  int64_t m, n;              // rows and columns of the product
+  int* status;
+  // logits
+  float factor;     // scale * log2(e)
+  const void* bias; // of the piece, or NULL
+  int bias_f32;
+  const int64_t* targets;
+  int64_t vocab, first; // first: vocabulary entry of column 0
+  int64_t ignore_index;
+  float2* partial; // EPI_LSE: [128-column block of the vocabulary][row]
+  float* picked;   // EPI_LSE: logit of the target, in units of log 2
+  const float* lse;
+  const float* grad;
+  int64_t grad_stride;
+  float scale;
+  __nv_bfloat16* slope;
+  int64_t slope_ld, slope_plane;
+  int planes;
+  float* sum; // EPI_SUM
+  int64_t sum_ld, sum_split;
+  int add;
+  void* out; // EPI_OUT
+  int64_t out_ld;
+  int out_f32, out_wide;
+};
+
+__device__ __forceinline__ float ex2(float x)
+{
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ bool counted(int64_t target, int64_t vocab, int64_t ignore_index)
+{
+  return target >= 0 && target < vocab && target != ignore_index;
+}
+
+// Which tile a work item is: the tiles of `group_m` row blocks go down the rows first, so that the
+// CTA pairs at work share a few column blocks (weights, read once) and the rows of the group stay in L2.
+__device__ __forceinline__ void locate(const GemmParams& P, int64_t item, int& split, int64_t& tm, int64_t& tn)
+{
+  const int64_t tiles = P.tiles_m * P.tiles_n;
+  split = (int)(item / tiles);
+  const int64_t tile = item - split * tiles, group = tile / (P.group_m * P.tiles_n);
+  const int64_t first = group * P.group_m, rest = tile - first * P.tiles_n;
+  const int64_t height = P.tiles_m - first < P.group_m ? P.tiles_m - first : P.group_m;
+  tn = rest / height;
+  tm = first + rest - tn * height;
+}
+
+__device__ __forceinline__ void range_of(const GemmParams& P, int split, int& begin, int& end)
+{
+  const int64_t total = (int64_t)P.kblocks * P.passes;
+  begin = (int)(total * split / P.splits), end = (int)(total * (split + 1) / P.splits);
+}
+
+// 32 logits of a row in units of log 2, -inf outside the vocabulary.
+__device__ __forceinline__ void logits32(const GemmParams& P, int64_t col, float (&v)[32])
+{
+  if (P.bias)
+  {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+    {
+      const int64_t c = col + i < P.n ? col + i : P.n - 1;
+      const float b = P.bias_f32 ? __ldg(static_cast<const float*>(P.bias) + c)
+                                 : __bfloat162float(static_cast<const __nv_bfloat16*>(P.bias)[c]);
+      v[i] = fmaf(v[i], P.factor, b * kLog2e);
+    }
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      v[i] *= P.factor;
+  }
+  if (col + 32 > P.n)
+  {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (col + i >= P.n)
+        v[i] = -INFINITY;
+  }
+}
+
+template <int EPI, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    vocab_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const GemmParams P)
+{
+  constexpr uint32_t kInstr = (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
+                              ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(kTile >> 3) << 17) |
+                              ((uint32_t)(kTile >> 4) << 24);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + kStages * kStageBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int64_t begin = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0)
+  {
+    for (int s = 0; s < kStages; ++s)
+    {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a)
+    {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kEpilogueWarps); // both CTAs' epilogue warps arrive on the leader's
+    }
+    *abort_flag = 0;
+    *reinterpret_cast<volatile long long*>(abort_flag + 2) = kWaitCyclesDefault;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1)
+  {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"((uint32_t)kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync_all(); // the peer's barriers are initialised before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t lead_full = mapa_u32(smem_u32(full), 0);
+  const uint32_t lead_tempty = mapa_u32(smem_u32(tempty), 0);
+  const uint32_t peer_empty = mapa_u32(smem_u32(empty), rank ^ 1);
+  const uint32_t peer_tfull = mapa_u32(smem_u32(tfull), rank ^ 1);
+
+  if (warp == 0)
+  {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0)
+    {
+      int s = 0;
+      uint32_t phase = 1;
+      bool alive = true;
+      for (int64_t item = begin; item < P.items && alive; item += step)
+      {
+        int split, it, it_end;
+        int64_t tm, tn;
+        locate(P, item, split, tm, tn);
+        range_of(P, split, it, it_end);
+        const int m0 = (int)(tm * kTile) + (int)rank * kRows, n0 = (int)(tn * kTile) + (int)rank * kRows;
+        int pass = it / P.kblocks, kb = it - pass * P.kblocks;
+        for (; it < it_end; ++it)
+        {
+          if (!mbar_wait_cluster(&empty[s], phase, abort_flag))
+          {
+            alive = false;
+            break;
+          }
+          if (leader)
+            mbar_expect_tx(&full[s], 2 * kStageBytes); // both CTAs' copies count on the leader's barrier
+          const uint32_t bar = lead_full + (uint32_t)(s * 8);
+          uint8_t* a = stages + s * kStageBytes;
+          uint8_t* b = a + kOperandBytes;
+          const int pa = (P.plane_a >> (4 * pass)) & 15, pb = (P.plane_b >> (4 * pass)) & 15;
+          const int k = kb * kDepth;
+          if (A_MN)
+          {
+            tma_load_3d_pair(a, &map_a, bar, m0, k, pa);
+            tma_load_3d_pair(a + kOperandBytes / 2, &map_a, bar, m0 + 64, k, pa);
+          }
+          else
+            tma_load_3d_pair(a, &map_a, bar, k, m0, pa);
+          if (B_MN)
+          {
+            tma_load_3d_pair(b, &map_b, bar, n0, k, pb);
+            tma_load_3d_pair(b + kOperandBytes / 2, &map_b, bar, n0 + 64, k, pb);
+          }
+          else
+            tma_load_3d_pair(b, &map_b, bar, k, n0, pb);
+          if (++kb == P.kblocks)
+            kb = 0, ++pass;
+          if (++s == kStages)
+            s = 0, phase ^= 1;
+        }
+      }
+      if (!alive)
+      {
+        // Let copies already in flight land before the CTA's shared memory goes away.
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL * kStages)
+        {
+        }
+      }
+    }
+  }
+  else if (warp == 1)
+  {
+    // ---------------------------------------------------------------- MMA issuer (the warp together, one lane issues)
+    if (leader)
+    {
+      // K-major: rows of 128 bytes, 8 to a swizzle atom.  MN-major: blocks of 64 columns (8 KB apart) of
+      // 64 k-rows, 8 k-rows to an atom, 16 k-rows to an instruction.
+      const uint64_t da0 = make_desc(smem_u32(stages), A_MN ? kOperandBytes / 2 : 16, 1024, 2);
+      const uint64_t db0 = make_desc(smem_u32(stages) + kOperandBytes, B_MN ? kOperandBytes / 2 : 16, 1024, 2);
+      constexpr uint32_t adv_a = (A_MN ? 2048 : 32) >> 4, adv_b = (B_MN ? 2048 : 32) >> 4;
+      int s = 0, turn = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int64_t item = begin; item < P.items && alive; item += step, ++turn)
+      {
+        const int acc = turn & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tempty[acc], ((turn >> 1) & 1) ^ 1, abort_flag)))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * kTile;
+        int it, it_end;
+        range_of(P, (int)(item / (P.tiles_m * P.tiles_n)), it, it_end);
+        for (uint32_t more = 0; it < it_end; ++it)
+        {
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[s], phase, abort_flag)))
+          {
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t sa = da0 + (uint64_t)(s * (kStageBytes >> 4)), sb = db0 + (uint64_t)(s * (kStageBytes >> 4));
+#pragma unroll
+          for (int ks = 0; ks < kDepth / 16; ++ks)
+          {
+            tc_mma_bf16_pair(d, sa + (uint64_t)(ks * adv_a), sb + (uint64_t)(ks * adv_b), kInstr, more);
+            more = 1;
+          }
+          tc_commit_pair(smem_u32(&empty[s])); // the stage is free in both CTAs
+          tc_commit_pair(peer_empty + (uint32_t)(s * 8));
+          if (++s == kStages)
+            s = 0, phase ^= 1;
+        }
+        if (alive)
+        {
+          tc_commit_pair(smem_u32(&tfull[acc]));
+          tc_commit_pair(peer_tfull + (uint32_t)(acc * 8));
+        }
+      }
+    }
+  }
+  else if (warp >= 4)
+  {
+    // ---------------------------------------------------------------- epilogue: a row a lane, 128 columns a warp
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    int turn = 0;
+    for (int64_t item = begin; item < P.items; item += step, ++turn)
+    {
+      int split;
+      int64_t tm, tn;
+      locate(P, item, split, tm, tn);
+      const int64_t row = tm * kTile + rank * kRows + quarter * 32 + lane;
+      const int64_t col0 = tn * kTile + half * 128;
+      const bool inside = row < P.m;
+      int64_t target = -1; // column of the target, outside the tile: not this one
+      bool count = false;
+      float lse2 = 0.0f, slope_scale = 0.0f;
+      if ((EPI == EPI_LSE || EPI == EPI_SLOPE) && inside)
+      {
+        const int64_t t = P.targets[row];
+        count = counted(t, P.vocab, P.ignore_index);
+        if (count)
+          target = t - P.first;
+        if (EPI == EPI_SLOPE && count)
+        {
+          lse2 = P.lse[row] * kLog2e;
+          slope_scale = P.grad[row * P.grad_stride] * P.scale;
+        }
+      }
+      const int acc = turn & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag)))
+        break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTile + half * 128;
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c)
+      {
+        const int64_t col = col0 + 32 * c;
+        float v[32];
+        __syncwarp();
+        tc_ld32(taddr + 32 * c, v);
+        if (EPI == EPI_LSE)
+        {
+          logits32(P, col, v);
+          if (target >= col && target < col + 32)
+          {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (target == col + i)
+                P.picked[row] = v[i];
+          }
+          float most = v[0];
+#pragma unroll
+          for (int i = 1; i < 32; ++i)
+            most = fmaxf(most, v[i]);
+          most = fmaxf(most, top);
+          // (nothing but -inf so far: zero in its place leaves the sum at 0, or NaN where a logit is NaN)
+          const float base = most == -INFINITY ? 0.0f : most;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            sum[i & 3] += ex2(v[i] - base);
+          total = fmaf(total, ex2(top - base), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+          top = most;
+        }
+        else if (EPI == EPI_SLOPE)
+        {
+          logits32(P, col, v);
+          const int hot = target >= col && target < col + 32 ? (int)(target - col) : -1;
+          // (past the last column of the piece: exp(-inf) = 0 is written, and nothing reads it)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+          {
+            const float p = ex2(v[i] - lse2) - (i == hot ? 1.0f : 0.0f);
+            v[i] = count ? slope_scale * p : 0.0f; // an ignored row is 0 whatever it holds
+          }
+          if (inside)
+          {
+            __nv_bfloat16* dst = P.slope + row * P.slope_ld + col;
+            for (int pl = 0; pl < P.planes; ++pl, dst += P.slope_plane)
+            {
+              float w[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2)
+              {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+                w[i / 2] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
+                v[i] -= __low2float(h), v[i + 1] -= __high2float(h);
+              }
+              st8(reinterpret_cast<float*>(dst), w);
+              st8(reinterpret_cast<float*>(dst) + 8, w + 8);
+            }
+          }
+        }
+        else if (EPI == EPI_SUM)
+        {
+          if (inside)
+          {
+            float* dst = P.sum + split * P.sum_split + row * P.sum_ld + col;
+            if (P.add)
+            {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+              {
+                float old[8];
+                ld8(dst + i, old);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  v[i + k] += old[k];
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              st8(dst + i, v + i);
+          }
+        }
+        else if (inside && col < P.n)
+        {
+          if (P.out_wide && col + 32 <= P.n)
+          {
+            if (P.out_f32)
+            {
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(P.out) + row * P.out_ld + col);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+            else
+            {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(P.out) + row * P.out_ld + col);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                dst[i] = pack8(v + 8 * i);
+            }
+          }
+          else
+          {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (col + i < P.n)
+              {
+                if (P.out_f32)
+                  static_cast<float*>(P.out)[row * P.out_ld + col + i] = v[i];
+                else
+                  static_cast<__nv_bfloat16*>(P.out)[row * P.out_ld + col + i] = __float2bfloat16_rn(v[i]);
+              }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive_cluster(lead_tempty + (uint32_t)(acc * 8));
+      if (EPI == EPI_LSE && inside)
+        P.partial[((P.first + col0) / 128) * P.m + row] = make_float2(top, total);
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all(); // neither CTA leaves while the other may still touch its memory
+  if (threadIdx.x == 0 && *abort_flag)
+    atomicExch(P.status, 1);
+  if (warp == 1)
+  {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemColumns)
+                 : "memory");
+  }
+}
+
+// lse and loss of every row from the parts.  A block joins `lanes` threads on each of 256 / lanes rows:
+// neighbouring threads read neighbouring rows of a part, and with few rows neighbouring parts.
+__global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restrict__ partial, int64_t parts, int64_t rows,
+                                                         int row_shift, const float* __restrict__ picked,
+                                                         const int64_t* __restrict__ targets, int64_t vocab,
+                                                         int64_t ignore_index, const int* __restrict__ status,
+                                                         float* __restrict__ loss, float* __restrict__ lse)
+{
+  __shared__ float tops[256], sums[256];
+  const int per = 1 << row_shift, r = threadIdx.x & (per - 1), lanes = 256 >> row_shift;
+  const int64_t row = ((int64_t)blockIdx.x << row_shift) + r;
+  float top = -INFINITY, total = 0.0f;
+  if (row < rows)
+    for (int64_t p = threadIdx.x >> row_shift; p < parts; p += lanes)
+    {
+      const float2 v = partial[p * rows + row];
+      const float most = fmaxf(top, v.x), base = most == -INFINITY ? 0.0f : most;
+      total = total * ex2(top - base) + v.y * ex2(v.x - base);
+      top = most;
+    }
+  tops[threadIdx.x] = top, sums[threadIdx.x] = total;
+  __syncthreads();
+  for (int half = lanes >> 1; half > 0; half >>= 1)
+  {
+    if ((int)(threadIdx.x >> row_shift) < half)
+    {
+      const int other = threadIdx.x + (half << row_shift);
+      const float a = tops[threadIdx.x], b = tops[other], most = fmaxf(a, b), base = most == -INFINITY ? 0.0f : most;
+      sums[threadIdx.x] = sums[threadIdx.x] * ex2(a - base) + sums[other] * ex2(b - base);
+      tops[threadIdx.x] = most;
+    }
+    __syncthreads();
+  }
+  if ((int)threadIdx.x < per && row < rows)
+  {
+    const bool count = counted(targets[row], vocab, ignore_index);
+    float l = tops[r] + log2f(sums[r]);
+    float d = l - (count ? picked[row] : 0.0f);
+    if (*status) // a device-side wait gave up: the parts are not complete
+      l = d = NAN;
+    lse[row] = count ? l * kLn2 : 0.0f;
+    loss[row] = count ? d * kLn2 : 0.0f;
+  }
+}
+
+// dst[plane][row][0..ld) = the planes of src[row][0..cols), zeros beyond; rows that do not count are zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_planes_kernel(const T* __restrict__ src, int64_t src_ld, int64_t rows,
+                                                           int64_t cols, __nv_bfloat16* __restrict__ dst, int64_t ld,
+                                                           int planes, const int64_t* __restrict__ targets,
+                                                           int64_t vocab, int64_t ignore_index)
+{
+  const int64_t chunks = ld / 8, total = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
+  {
+    const int64_t row = i / chunks, col = (i - row * chunks) * 8;
+    float v[8];
+    const bool keep = !targets || counted(targets[row], vocab, ignore_index);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      v[k] = keep && col + k < cols ? to_float(src[row * src_ld + col + k]) : 0.0f;
+    for (int pl = 0; pl < planes; ++pl)
+    {
+      const uint4 h = pack8(v);
+      *reinterpret_cast<uint4*>(dst + ((int64_t)pl * rows + row) * ld + col) = h;
+      float back[8];
+      unpack8(h, back);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] -= back[k];
+    }
+  }
+}
+
+// out[row][col] = the sum of the splits' sums, in the type of the tensors.
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict__ sum, int64_t ld, int64_t split_stride,
+                                                        int splits, int64_t rows, int64_t cols, T* __restrict__ out,
+                                                        int64_t out_ld, const int* __restrict__ status)
+{
+  const float poison = *status ? NAN : 0.0f;
+  const int64_t chunks = (cols + 3) / 4, total = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
+  {
+    const int64_t row = i / chunks, col = (i - row * chunks) * 4;
+    float4 v = make_float4(poison, poison, poison, poison);
+    for (int s = 0; s < splits; ++s)
+    {
+      const float4 w = *reinterpret_cast<const float4*>(sum + s * split_stride + row * ld + col);
+      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < cols)
+        out[row * out_ld + col + k] = from_float<T>(f[k]);
+  }
+}
+
+// out[col] = factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
+                                                            int64_t plane, int planes, int64_t rows, int64_t cols,
+                                                            float factor, T* __restrict__ out,
+                                                            const int* __restrict__ status)
+{
+  __shared__ float2 parts[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col = (int64_t)blockIdx.x * 64 + 2 * lane; // (ld is a multiple of 256: always inside a row)
+  float2 total = make_float2(0.0f, 0.0f);
+  for (int64_t row = warp; row < rows; row += 8)
+    for (int pl = planes - 1; pl >= 0; --pl)
+    {
+      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(slope + pl * plane + row * ld + col));
+      total.x += v.x, total.y += v.y;
+    }
+  parts[warp][lane] = total;
+  __syncthreads();
+  if (warp == 0)
+  {
+    total = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < 8; ++w)
+      total.x += parts[w][lane].x, total.y += parts[w][lane].y;
+    const float poison = *status ? NAN : 0.0f;
+    if (col < cols)
+      out[col] = from_float<T>(fmaf(total.x, factor, poison));
+    if (col + 1 < cols)
+      out[col + 1] = from_float<T>(fmaf(total.y, factor, poison));
+  }
+}
+
+// ------------------------------------------------------------------------------ host
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
+
+// bf16 operand [planes][rows][cols] in 128-byte swizzled boxes of 64 columns.
+int operand_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int planes, int64_t plane,
+                int box_rows)
+{
+  EncodeTiledFn fn = encode_fn();
+  if (!fn)
+    return dpc::fail(DPC_ERR_CUDA, "vocabulary loss: the driver has no tensor-map encoder");
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+  cuuint32_t box[3] = {kDepth, (cuuint32_t)box_rows, 1}, unit[3] = {1, 1, 1};
+  if (fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, unit,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return dpc::fail(DPC_ERR_CUDA, "vocabulary loss: the driver refused a tensor map");
+  return DPC_OK;
+}
+
+// One operand of a product: a matrix of bf16 planes with the contraction along its columns (K-major)
+// or along its rows.
+struct Operand
+{
+  const void* base;
+  int64_t cols, rows, ld, plane;
+};
+
+template <int EPI, bool A_MN, bool B_MN>
+int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, int planes, int64_t m, int64_t n,
+            int64_t contraction, GemmParams P)
+{
+  CUtensorMap map_a, map_b;
+  if (int rc = operand_map(&map_a, a.base, a.cols, a.rows, a.ld, planes, a.plane, A_MN ? kDepth : kRows))
+    return rc;
+  if (int rc = operand_map(&map_b, b.base, b.cols, b.rows, b.ld, planes, b.plane, B_MN ? kDepth : kRows))
+    return rc;
+  P.m = m, P.n = n;
+  P.tiles_m = ceil_div(m, kTile), P.tiles_n = ceil_div(n, kTile);
+  P.group_m = std::min<int64_t>(P.tiles_m, 32);
+  P.kblocks = (int)ceil_div(contraction, kDepth);
+  // Plane pairs of a pass, smallest terms first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
+  P.passes = planes == 3 ? 6 : 1;
+  P.plane_a = planes == 3 ? 0x001102u : 0u;
+  P.plane_b = planes == 3 ? 0x010120u : 0u;
+  P.splits = (int)std::min<int64_t>(P.splits, (int64_t)P.kblocks * P.passes);
+  P.items = P.tiles_m * P.tiles_n * P.splits;
+  P.planes = planes;
+  auto kernel = vocab_product_kernel<EPI, A_MN, B_MN>;
+  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  const int blocks = 2 * (int)std::min<int64_t>(P.items, pairs);
+  kernel<<<blocks, kThreads, kSmemBytes, stream>>>(map_a, map_b, P);
+  return launched("vocab_product_kernel");
+}
+
+struct Layout
+{
+  int pairs = 0, planes = 1, splits = 1;
+  bool copy_hidden = false, copy_weight = false;
+  int64_t kp = 0;    // columns of the copies
+  int64_t ks = 0;    // columns of the sums of d_hidden
+  int64_t piece = 0; // vocabulary entries at a time, a multiple of the tile (or all of them)
+  size_t status = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
+};
+
+bool tma_ready(const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
+
+int check(const dpc_vocab_ce* c, bool backward, const char* who)
+{
+  const std::string name = who;
+  if (!c)
+    return dpc::fail(DPC_ERR_INVALID, name + ": no description");
+  if (c->type != DPC_TYPE_F32 && c->type != DPC_TYPE_BF16)
+    return dpc::fail(DPC_ERR_INVALID, name + ": type is neither DPC_TYPE_F32 nor DPC_TYPE_BF16");
+  if (c->rows < 0 || c->width < 1 || c->vocab < 1)
+    return dpc::fail(DPC_ERR_INVALID, name + ": rows >= 0, width >= 1 and vocab >= 1 are needed");
+  const int64_t most = (int64_t)1 << 28;
+  if (c->rows > most || c->width > most || c->vocab > most)
+    return dpc::fail(DPC_ERR_TOO_LARGE, name + ": rows, width and vocab may be 2^28 at most");
+  if (c->hidden_stride < c->width || c->weight_stride < c->width || c->hidden_stride > most || c->weight_stride > most)
+    return dpc::fail(DPC_ERR_INVALID, name + ": a row stride is smaller than the width (or above 2^28)");
+  if (!(c->scale > 0.0f) || !std::isfinite(c->scale))
+    return dpc::fail(DPC_ERR_INVALID, name + ": scale has to be positive and finite");
+  if (backward && (c->grad_stride != 0 && c->grad_stride != 1))
+    return dpc::fail(DPC_ERR_INVALID, name + ": grad_stride is 1, or 0 for one gradient for all rows");
+  if (backward && (c->d_hidden_stride < c->width || c->d_weight_stride < c->width || c->d_hidden_stride > most ||
+                   c->d_weight_stride > most))
+    return dpc::fail(DPC_ERR_INVALID, name + ": a gradient's row stride is smaller than the width (or above 2^28)");
+  return DPC_OK;
+}
+
+int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
+{
+  int device = 0, sms = 0;
+  DPC_CUDA(cudaGetDevice(&device));
+  DPC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  L.pairs = std::max(1, sms / 2);
+  L.planes = c->type == DPC_TYPE_F32 ? 3 : 1;
+  // (backward: the rows that do not count are zeros in the copy, so that an infinity in one of them
+  // does not reach d_weight as 0 * inf)
+  L.copy_hidden = backward || L.planes > 1 || !tma_ready(c->hidden, c->hidden_stride);
+  L.copy_weight = L.planes > 1 || !tma_ready(c->weight, c->weight_stride);
+  L.kp = round_up(c->width, 8);
+  L.ks = round_up(c->width, kTile);
+  const int64_t all = round_up(c->vocab, kTile);
+  L.piece = all;
+  auto limit = [&](int64_t bytes_each) {
+    L.piece = std::min(L.piece, std::max<int64_t>(kTile, (int64_t)(kPieceBytes / bytes_each) / kTile * kTile));
+  };
+  if (L.copy_weight)
+    limit(L.kp * 2 * L.planes);
+  if (backward)
+    limit(std::max<int64_t>(1, c->rows) * 2 * L.planes);
+  L.piece = round_up(ceil_div(all, ceil_div(all, L.piece)), kTile); // pieces of like size
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  L.status = take(sizeof(int));
+  if (L.copy_hidden)
+    L.hidden = take((size_t)c->rows * L.kp * 2 * L.planes);
+  if (L.copy_weight)
+    L.weight = take((size_t)std::min(L.piece, c->vocab) * L.kp * 2 * L.planes);
+  if (backward)
+  {
+    // Few tiles of d_hidden: the contraction over the piece is shared out, 4 blocks of it at least each.
+    const int64_t tiles = ceil_div(c->rows, kTile) * (L.ks / kTile);
+    const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth) * (L.planes == 3 ? 6 : 1);
+    L.splits = (int)std::max<int64_t>(1, std::min(L.pairs / std::max<int64_t>(1, tiles), blocks / 4));
+    L.slope = take((size_t)c->rows * L.piece * 2 * L.planes);
+    L.sum = take((size_t)L.splits * c->rows * L.ks * sizeof(float));
+  }
+  else
+  {
+    L.partial = take((size_t)(all / 128) * c->rows * sizeof(float2));
+    L.picked = take((size_t)c->rows * sizeof(float));
+  }
+  L.bytes = at;
+  return DPC_OK;
+}
+
+int workspace_ok(const dpc_vocab_ce* c, const Layout& L, const char* who)
+{
+  if (!c->workspace || reinterpret_cast<uintptr_t>(c->workspace) % 256)
+    return dpc::fail(DPC_ERR_INVALID, std::string(who) + ": the workspace has to be device memory on a 256-byte boundary");
+  if (c->workspace_bytes < L.bytes)
+    return dpc::fail(DPC_ERR_INVALID, std::string(who) + ": the workspace has " + std::to_string(c->workspace_bytes) +
+                                          " bytes, " + std::to_string(L.bytes) + " are needed");
+  return DPC_OK;
+}
+
+int grid_for(int64_t work)
+{
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(work, 256), 148 * 16));
+}
+
+int make_planes(cudaStream_t stream, const dpc_vocab_ce* c, const void* src, int64_t src_ld, int64_t rows,
+                const Layout& L, void* dst, bool mask)
+{
+  const int64_t* targets = mask ? c->targets : nullptr;
+  __nv_bfloat16* to = static_cast<__nv_bfloat16*>(dst);
+  const int blocks = grid_for(rows * (L.kp / 8));
+  if (c->type == DPC_TYPE_F32)
+    vocab_planes_kernel<float><<<blocks, 256, 0, stream>>>(static_cast<const float*>(src), src_ld, rows, c->width, to,
+                                                           L.kp, L.planes, targets, c->vocab, c->ignore_index);
+  else
+    vocab_planes_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), src_ld, rows,
+                                                                   c->width, to, L.kp, L.planes, targets, c->vocab,
+                                                                   c->ignore_index);
+  return launched("vocab_planes_kernel");
+}
+
+const void* at_row(const void* p, int type, int64_t elements)
+{
+  return static_cast<const char*>(p) + elements * (type == DPC_TYPE_F32 ? 4 : 2);
+}
+
+// Operands of a piece of the vocabulary that starts at `first`; its weights are brought into planes here.
+int piece_weight(cudaStream_t stream, const dpc_vocab_ce* c, const Layout& L, int64_t first, int64_t count, char* ws,
+                 Operand& weight)
+{
+  const void* src = at_row(c->weight, c->type, first * c->weight_stride);
+  if (!L.copy_weight)
+  {
+    weight = {src, c->width, count, c->weight_stride, count * c->weight_stride};
+    return DPC_OK;
+  }
+  weight = {ws + L.weight, c->width, count, L.kp, count * L.kp};
+  return make_planes(stream, c, src, c->weight_stride, count, L, ws + L.weight, false);
+}
+
+int prepare_hidden(cudaStream_t stream, const dpc_vocab_ce* c, const Layout& L, bool mask, char* ws, Operand& hidden)
+{
+  if (!L.copy_hidden)
+  {
+    hidden = {c->hidden, c->width, c->rows, c->hidden_stride, c->rows * c->hidden_stride};
+    return DPC_OK;
+  }
+  hidden = {ws + L.hidden, c->width, c->rows, L.kp, c->rows * L.kp};
+  return make_planes(stream, c, c->hidden, c->hidden_stride, c->rows, L, ws + L.hidden, mask);
+}
+
+GemmParams base_params(const dpc_vocab_ce* c, const Layout& L, int64_t first, char* ws)
+{
+  GemmParams P = {};
+  P.splits = 1;
+  P.status = reinterpret_cast<int*>(ws + L.status);
+  P.factor = c->scale * kLog2e;
+  P.scale = c->scale;
+  P.bias = c->bias ? at_row(c->bias, c->type, first) : nullptr;
+  P.bias_f32 = c->type == DPC_TYPE_F32;
+  P.targets = c->targets;
+  P.vocab = c->vocab, P.first = first, P.ignore_index = c->ignore_index;
+  return P;
+}
+
+int forward(cudaStream_t stream, const dpc_vocab_ce* c)
+{
+  const char* who = "dpc_vocab_ce_forward";
+  if (int rc = check(c, false, who))
+    return rc;
+  if (c->rows == 0)
+    return DPC_OK;
+  if (!c->hidden || !c->weight || !c->targets || !c->loss || !c->lse)
+    return dpc::fail(DPC_ERR_INVALID, std::string(who) + ": null pointer");
+  Layout L;
+  if (int rc = lay_out(c, false, L))
+    return rc;
+  if (int rc = workspace_ok(c, L, who))
+    return rc;
+  char* ws = static_cast<char*>(c->workspace);
+  DPC_CUDA(cudaMemsetAsync(ws + L.status, 0, sizeof(int), stream));
+  Operand hidden, weight;
+  if (int rc = prepare_hidden(stream, c, L, false, ws, hidden))
+    return rc;
+  for (int64_t first = 0; first < c->vocab; first += L.piece)
+  {
+    const int64_t count = std::min(L.piece, c->vocab - first);
+    if (int rc = piece_weight(stream, c, L, first, count, ws, weight))
+      return rc;
+    GemmParams P = base_params(c, L, first, ws);
+    P.partial = reinterpret_cast<float2*>(ws + L.partial);
+    P.picked = reinterpret_cast<float*>(ws + L.picked);
+    if (int rc = product<EPI_LSE, false, false>(stream, L.pairs, hidden, weight, L.planes, c->rows, count, c->width, P))
+      return rc;
+  }
+  int row_shift = 0;
+  while (row_shift < 5 && ((int64_t)1 << row_shift) < c->rows)
+    ++row_shift;
+  vocab_join_kernel<<<(unsigned)ceil_div(c->rows, (int64_t)1 << row_shift), 256, 0, stream>>>(
+      reinterpret_cast<const float2*>(ws + L.partial), round_up(c->vocab, kTile) / 128, c->rows, row_shift,
+      reinterpret_cast<const float*>(ws + L.picked), c->targets, c->vocab, c->ignore_index,
+      reinterpret_cast<const int*>(ws + L.status), c->loss, c->lse);
+  return launched("vocab_join_kernel");
+}
+
+int zero_rows(cudaStream_t stream, void* p, int type, int64_t stride, int64_t width, int64_t rows)
+{
+  const size_t size = type == DPC_TYPE_F32 ? 4 : 2;
+  DPC_CUDA(cudaMemset2DAsync(p, stride * size, 0, width * size, rows, stream));
+  return DPC_OK;
+}
+
+int backward(cudaStream_t stream, const dpc_vocab_ce* c)
+{
+  const char* who = "dpc_vocab_ce_backward";
+  if (int rc = check(c, true, who))
+    return rc;
+  if (!c->d_weight || (c->d_bias && !c->bias))
+    return dpc::fail(DPC_ERR_INVALID, std::string(who) + ": null pointer");
+  if (c->rows == 0)
+  {
+    if (c->d_bias)
+      if (int rc = zero_rows(stream, c->d_bias, c->type, c->vocab, c->vocab, 1))
+        return rc;
+    return zero_rows(stream, c->d_weight, c->type, c->d_weight_stride, c->width, c->vocab);
+  }
+  if (!c->hidden || !c->weight || !c->targets || !c->lse || !c->grad_loss || !c->d_hidden)
+    return dpc::fail(DPC_ERR_INVALID, std::string(who) + ": null pointer");
+  Layout L;
+  if (int rc = lay_out(c, true, L))
+    return rc;
+  if (int rc = workspace_ok(c, L, who))
+    return rc;
+  char* ws = static_cast<char*>(c->workspace);
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  float* sum = reinterpret_cast<float*>(ws + L.sum);
+  __nv_bfloat16* slope = reinterpret_cast<__nv_bfloat16*>(ws + L.slope);
+  DPC_CUDA(cudaMemsetAsync(status, 0, sizeof(int), stream));
+  Operand hidden, weight;
+  if (int rc = prepare_hidden(stream, c, L, true, ws, hidden))
+    return rc;
+  const int64_t plane = c->rows * L.piece;
+  for (int64_t first = 0; first < c->vocab; first += L.piece)
+  {
+    const int64_t count = std::min(L.piece, c->vocab - first);
+    if (int rc = piece_weight(stream, c, L, first, count, ws, weight))
+      return rc;
+    GemmParams P = base_params(c, L, first, ws);
+    P.lse = c->lse, P.grad = c->grad_loss, P.grad_stride = c->grad_stride;
+    P.slope = slope, P.slope_ld = L.piece, P.slope_plane = plane;
+    if (int rc = product<EPI_SLOPE, false, false>(stream, L.pairs, hidden, weight, L.planes, c->rows, count, c->width, P))
+      return rc;
+    const Operand s = {slope, count, c->rows, L.piece, plane};
+    P = base_params(c, L, first, ws);
+    P.splits = L.splits;
+    P.sum = sum, P.sum_ld = L.ks, P.sum_split = c->rows * L.ks, P.add = first > 0;
+    if (int rc = product<EPI_SUM, false, true>(stream, L.pairs, s, weight, L.planes, c->rows, c->width, count, P))
+      return rc;
+    P = base_params(c, L, first, ws);
+    P.out = const_cast<void*>(at_row(c->d_weight, c->type, first * c->d_weight_stride));
+    P.out_ld = c->d_weight_stride, P.out_f32 = c->type == DPC_TYPE_F32;
+    P.out_wide = reinterpret_cast<uintptr_t>(P.out) % 16 == 0 && c->d_weight_stride % (P.out_f32 ? 4 : 8) == 0;
+    if (int rc = product<EPI_OUT, true, true>(stream, L.pairs, s, hidden, L.planes, count, c->width, c->rows, P))
+      return rc;
+    if (c->d_bias)
+    {
+      const unsigned blocks = (unsigned)ceil_div(count, 64);
+      if (c->type == DPC_TYPE_F32)
+        vocab_columns_kernel<float><<<blocks, 256, 0, stream>>>(slope, L.piece, plane, L.planes, c->rows, count,
+                                                                1.0f / c->scale, static_cast<float*>(c->d_bias) + first,
+                                                                status);
+      else
+        vocab_columns_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(
+            slope, L.piece, plane, L.planes, c->rows, count, 1.0f / c->scale,
+            static_cast<__nv_bfloat16*>(c->d_bias) + first, status);
+      if (int rc = launched("vocab_columns_kernel"))
+        return rc;
+    }
+  }
+  const int blocks = grid_for(c->rows * ceil_div(c->width, 4));
+  if (c->type == DPC_TYPE_F32)
+    vocab_sum_kernel<float><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
+                                                        static_cast<float*>(c->d_hidden), c->d_hidden_stride, status);
+  else
+    vocab_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
+                                                                static_cast<__nv_bfloat16*>(c->d_hidden),
+                                                                c->d_hidden_stride, status);
+  return launched("vocab_sum_kernel");
+}
+} // namespace
+
+int dpc_vocab_ce_workspace(const dpc_vocab_ce* c, int backward, size_t* bytes)
+{
+  return guarded("dpc_vocab_ce_workspace", [&] {
+    if (!bytes)
+      return dpc::fail(DPC_ERR_INVALID, "dpc_vocab_ce_workspace: null pointer");
+    if (int rc = check(c, backward != 0, "dpc_vocab_ce_workspace"))
+      return rc;
+    Layout L;
+    if (int rc = lay_out(c, backward != 0, L))
+      return rc;
+    *bytes = L.bytes;
+    return (int)DPC_OK;
+  });
+}
+
+int dpc_vocab_ce_forward(void* stream, const dpc_vocab_ce* c)
+{
+  return guarded("dpc_vocab_ce_forward", [&] { return forward(static_cast<cudaStream_t>(stream), c); });
+}
+
+int dpc_vocab_ce_backward(void* stream, const dpc_vocab_ce* c)
+{
+  return guarded("dpc_vocab_ce_backward", [&] { return backward(static_cast<cudaStream_t>(stream), c); });
+}

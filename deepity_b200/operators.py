@@ -1,0 +1,356 @@
+"""Operators of deep stacks with large outputs, on CUDA ``torch`` tensors.
+
+    new, normed, stats = residual_norm(stream, branch, gate=gate, post_weight=wp, pre_weight=wn)
+    out, packed = activate_and_pack(preact, "gelu")
+    loss, lse = vocab_cross_entropy(normed, weight, targets)
+
+Each has an explicit gradient (``residual_norm_backward``, ``packed_activation_backward``,
+``vocab_cross_entropy_backward``): like the layers of this package, and unlike torch's own functions,
+they record nothing for automatic differentiation, and their results carry no history.
+
+Tensors are float32 or bfloat16, all of a call alike, on one device.  Leading dimensions are free and count as
+rows, as far as one stride describes them; the last dimension is contiguous.  Work is enqueued on torch's current
+stream of the tensors' device; results and workspaces come from torch's allocator, so that calls can be
+captured into CUDA graphs and made on several streams at once.  Nothing waits for the GPU.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+from . import _lib
+from .layer import ACT_IDS, Activation
+
+BLOCK = 128  # elements of a row that share a scale
+_NORMS = {"rms": 0, "layer": 1}
+
+
+def _torch():
+    import torch
+    return torch
+
+
+class _Call:
+    """What the tensors of one call have in common: type and device, taken from the first."""
+
+    def __init__(self, name, first_name, first):
+        torch = _torch()
+        self.torch, self.name = torch, name
+        if not torch.is_tensor(first):
+            raise TypeError(f"{name}: {first_name} has to be a torch tensor, not {type(first).__name__}")
+        if first.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"{name}: {first_name} is {first.dtype}; float32 and bfloat16 are supported")
+        if not first.is_cuda:
+            raise ValueError(f"{name}: {first_name} is on {first.device}; there is no CPU path")
+        self.dtype, self.device = first.dtype, first.device
+        self.type = 0 if first.dtype == torch.float32 else 1
+
+    def tensor(self, label, t, dtype=None):
+        if not self.torch.is_tensor(t):
+            raise TypeError(f"{self.name}: {label} has to be a torch tensor, not {type(t).__name__}")
+        if t.dtype != (dtype or self.dtype):
+            raise TypeError(f"{self.name}: {label} is {t.dtype}, {dtype or self.dtype} is needed")
+        if t.device != self.device:
+            raise ValueError(f"{self.name}: {label} is on {t.device}, the call on {self.device}")
+        return t
+
+    def matrix(self, label, t, shape=None):
+        """(rows, width, row stride) of a tensor whose leading dimensions one stride describes."""
+        t = self.tensor(label, t)
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{self.name}: {label} is {tuple(t.shape)}, {tuple(shape)} is needed")
+        if t.dim() < 2:
+            raise ValueError(f"{self.name}: {label} needs two dimensions at least, it has {t.dim()}")
+        rows, width = math.prod(t.shape[:-1]), t.shape[-1]
+        if width > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{self.name}: the last dimension of {label} has to be contiguous")
+        try:
+            stride = t.view(rows, width).stride(0)
+        except RuntimeError:
+            raise ValueError(f"{self.name}: no one stride describes the rows of {label}: make it contiguous") from None
+        return rows, width, max(width, 1) if rows <= 1 else stride
+
+    def vector(self, label, t, width):
+        if t is None:
+            return None
+        if tuple(self.tensor(label, t).shape) != (width,) or (width > 1 and t.stride(0) != 1):
+            raise ValueError(f"{self.name}: {label} has to be a contiguous vector of {width}")
+        return t.data_ptr()
+
+    def empty(self, *shape, dtype=None):
+        return self.torch.empty(*shape, dtype=dtype or self.dtype, device=self.device)
+
+    def workspace(self, size_of, *args):
+        size = ctypes.c_size_t()
+        _lib.check(size_of(*args, ctypes.byref(size)))
+        return self.empty(size.value, dtype=self.torch.uint8)
+
+    def current(self):
+        return self.torch.cuda.device(self.device)
+
+    def stream(self):
+        return self.torch.cuda.current_stream(self.device).cuda_stream
+
+
+# ------------------------------------------------------------------------------ vocabulary loss
+class VocabGradients(NamedTuple):
+    hidden: object
+    weight: object
+    bias: Optional[object]
+
+
+def _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index):
+    torch = call.torch
+    rows, width, hidden_stride = call.matrix("hidden", hidden)
+    if call.tensor("weight", weight).dim() != 2 or weight.shape[1] != width:
+        raise ValueError(f"{call.name}: weight is {tuple(weight.shape)}, (vocabulary, {width}) is needed")
+    vocab, _, weight_stride = call.matrix("weight", weight)
+    if call.tensor("targets", targets, torch.int64).shape != hidden.shape[:-1]:
+        raise ValueError(f"{call.name}: targets is {tuple(targets.shape)}, {tuple(hidden.shape[:-1])} is needed")
+    targets = targets.contiguous()
+    c = _lib.VocabCe(rows=rows, width=width, vocab=vocab, hidden_stride=hidden_stride, weight_stride=weight_stride,
+                     type=call.type, scale=scale, ignore_index=ignore_index, hidden=hidden.data_ptr(),
+                     weight=weight.data_ptr(), bias=call.vector("bias", bias, vocab), targets=targets.data_ptr())
+    return c, targets
+
+
+def vocab_cross_entropy(hidden, weight, targets, bias=None, *, scale: float = 1.0, ignore_index: int = -100):
+    """Softmax cross entropy of ``hidden`` [..., width] against a vocabulary ``weight`` [vocab, width], without
+    ever keeping the logits ``scale * hidden @ weight.T + bias``.
+
+    Returns ``(loss, lse)``, float32 of ``targets``' shape: the loss of every row and the logarithm of its sum of
+    exponentials, which ``vocab_cross_entropy_backward`` needs.  Rows whose target (int64) is ``ignore_index`` or
+    outside the vocabulary are ignored: both are 0, whatever the row holds."""
+    call = _Call("vocab_cross_entropy", "hidden", hidden)
+    c, targets = _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index)
+    lib = _lib.load()
+    loss = call.empty(targets.shape, dtype=call.torch.float32)
+    lse = call.empty(targets.shape, dtype=call.torch.float32)
+    c.loss, c.lse = loss.data_ptr(), lse.data_ptr()
+    with call.current():
+        ws = call.workspace(lib.dpc_vocab_ce_workspace, ctypes.byref(c), 0)
+        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.dpc_vocab_ce_forward(call.stream(), ctypes.byref(c)))
+    return loss, lse
+
+
+def vocab_cross_entropy_backward(grad_loss, hidden, weight, targets, lse, bias=None, *, scale: float = 1.0,
+                                 ignore_index: int = -100) -> VocabGradients:
+    """Gradients of ``vocab_cross_entropy`` with respect to hidden, weight and bias (None without one), in
+    their type.  ``grad_loss``: float32, the gradient of every row's loss, or one value for all rows; ``lse``
+    as the forward call returned it."""
+    call = _Call("vocab_cross_entropy_backward", "hidden", hidden)
+    torch = call.torch
+    c, targets = _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index)
+    lib = _lib.load()
+    if call.tensor("lse", lse, torch.float32).shape != targets.shape:
+        raise ValueError(f"{call.name}: lse is {tuple(lse.shape)}, {tuple(targets.shape)} is needed")
+    call.tensor("grad_loss", grad_loss, torch.float32)
+    if grad_loss.numel() != 1 and grad_loss.shape != targets.shape:
+        raise ValueError(f"{call.name}: grad_loss is {tuple(grad_loss.shape)}, {tuple(targets.shape)} or one value is needed")
+    one = grad_loss.numel() == 1 or (grad_loss.numel() > 1 and not any(grad_loss.stride()))
+    grad_loss, lse = grad_loss if one else grad_loss.contiguous(), lse.contiguous()
+    d_hidden, d_weight = call.empty(hidden.shape), call.empty(weight.shape)
+    d_bias = None if bias is None else call.empty(bias.shape)
+    c.lse, c.grad_loss, c.grad_stride = lse.data_ptr(), grad_loss.data_ptr(), 0 if one else 1
+    c.d_hidden, c.d_hidden_stride = d_hidden.data_ptr(), c.width
+    c.d_weight, c.d_weight_stride = d_weight.data_ptr(), c.width
+    c.d_bias = None if bias is None else d_bias.data_ptr()
+    with call.current():
+        ws = call.workspace(lib.dpc_vocab_ce_workspace, ctypes.byref(c), 1)
+        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.dpc_vocab_ce_backward(call.stream(), ctypes.byref(c)))
+    return VocabGradients(d_hidden, d_weight, d_bias)
+
+
+# ------------------------------------------------------------------------------ residual norms
+class ResidualNormGradients(NamedTuple):
+    stream: object
+    branch: Optional[object]
+    gate: Optional[object]
+    post_weight: Optional[object]
+    post_bias: Optional[object]
+    pre_weight: Optional[object]
+    pre_bias: Optional[object]
+
+
+def _norm_call(call, like, branch, norm, post_norm, post_weight, post_bias, gate, stream_scale, branch_scale,
+               pre_weight, pre_bias, eps):
+    if norm not in _NORMS:
+        raise ValueError(f"{call.name}: norm {norm!r} is none of {sorted(_NORMS)}")
+    rows, width, _ = call.matrix("the residual stream", like)
+    post_norm = post_weight is not None or post_bias is not None if post_norm is None else bool(post_norm)
+    c = _lib.ResidualNorm(rows=rows, width=width, groups=1, type=call.type, norm=_NORMS[norm], post_norm=post_norm,
+                          stream_scale=stream_scale, branch_scale=branch_scale, eps=eps,
+                          post_weight=call.vector("post_weight", post_weight, width),
+                          post_bias=call.vector("post_bias", post_bias, width),
+                          pre_weight=call.vector("pre_weight", pre_weight, width),
+                          pre_bias=call.vector("pre_bias", pre_bias, width))
+    if branch is not None:
+        c.branch_stride = call.matrix("branch", branch, like.shape)[2]
+        c.branch = branch.data_ptr()
+    elif post_norm or gate is not None or stream_scale != 1.0:
+        raise ValueError(f"{call.name}: without a branch there is no gate, post norm or stream scale")
+    if gate is not None:
+        table = call.tensor("gate", gate)
+        table = table[None] if table.dim() == 1 else table
+        c.groups, gate_width, c.gate_stride = call.matrix("gate", table)
+        if gate_width != width or c.groups < 1 or rows % c.groups:
+            raise ValueError(f"{call.name}: gate is {tuple(gate.shape)}; its last dimension has to be {width}, and "
+                             f"its rows have to divide {rows}")
+        c.gate = gate.data_ptr()
+    if rows == 0:  # empty tensors have no addresses: the presence of each operand is what counts
+        c.branch = None if branch is None else 16
+        c.gate = None if gate is None else 16
+    return c
+
+
+def residual_norm(stream, branch=None, *, norm: str = "rms", post_norm: Optional[bool] = None, post_weight=None,
+                  post_bias=None, gate=None, stream_scale: float = 1.0, branch_scale: float = 1.0, pre_weight=None,
+                  pre_bias=None, eps: float = 1e-6):
+    """The end of one residual block and the norm before the next, in one pass:
+
+        new_stream = stream_scale * stream + branch_scale * gate * (norm(branch) * post_weight + post_bias)
+        normed = norm(new_stream) * pre_weight + pre_bias
+
+    ``stream`` and ``branch`` [..., width]; ``norm``: "rms" or "layer"; ``post_norm=False`` (the default without
+    post weights) takes the branch as it is.  ``gate``: [width], or [groups, width] (also [..., width]) for as many equal
+    runs of rows, e.g. one of a sequence.  Without a branch (before the first block) new_stream is ``stream`` itself.
+
+    Returns ``(new_stream, normed, stats)``; ``stats`` (float32 [..., 4]: mean and 1/deviation of the branch and of the new stream)
+    goes to ``residual_norm_backward`` with ``new_stream`` and ``branch``."""
+    call = _Call("residual_norm", "stream", stream)
+    c = _norm_call(call, stream, branch, norm, post_norm, post_weight, post_bias, gate, stream_scale, branch_scale,
+                   pre_weight, pre_bias, eps)
+    lib = _lib.load()
+    c.stream, c.stream_stride = stream.data_ptr(), call.matrix("stream", stream)[2]
+    new_stream = stream if branch is None else call.empty(stream.shape)
+    normed = call.empty(stream.shape)
+    stats = call.empty(*stream.shape[:-1], 4, dtype=call.torch.float32)
+    if branch is not None:
+        c.new_stream, c.new_stream_stride = new_stream.data_ptr(), c.width
+    c.normed, c.normed_stride, c.stats = normed.data_ptr(), c.width, stats.data_ptr()
+    with call.current():
+        _lib.check(lib.dpc_residual_norm_forward(call.stream(), ctypes.byref(c)))
+    return new_stream, normed, stats
+
+
+def residual_norm_backward(d_normed, d_stream, new_stream, branch, stats, *, norm: str = "rms",
+                           post_norm: Optional[bool] = None, post_weight=None, post_bias=None, gate=None,
+                           stream_scale: float = 1.0, branch_scale: float = 1.0, pre_weight=None,
+                           pre_bias=None) -> ResidualNormGradients:
+    """Gradients of ``residual_norm`` from those of ``normed`` and of the new stream (``d_stream``; None where nothing
+    else reads it), with the tensors and options of the forward call.  What was not given has None."""
+    call = _Call("residual_norm_backward", "new_stream", new_stream)
+    c = _norm_call(call, new_stream, branch, norm, post_norm, post_weight, post_bias, gate, stream_scale, branch_scale,
+                   pre_weight, pre_bias, 0.0)
+    lib, shape, width = _lib.load(), new_stream.shape, c.width
+    c.new_stream, c.new_stream_stride = new_stream.data_ptr(), call.matrix("new_stream", new_stream)[2]
+    c.d_normed_stride = call.matrix("d_normed", d_normed, shape)[2]
+    c.d_normed = d_normed.data_ptr()
+    if d_stream is not None:
+        c.d_new_stream_stride = call.matrix("d_stream", d_stream, shape)[2]
+        c.d_new_stream = d_stream.data_ptr()
+    if tuple(call.tensor("stats", stats, call.torch.float32).shape) != (*shape[:-1], 4) or not stats.is_contiguous():
+        raise ValueError(f"{call.name}: stats has to be the tensor that residual_norm returned")
+    c.stats = stats.data_ptr()
+    d_in = call.empty(shape)
+    c.d_stream, c.d_stream_stride = d_in.data_ptr(), width
+    d_branch = None if branch is None else call.empty(shape)
+    if branch is not None:
+        c.d_branch, c.d_branch_stride = (d_branch.data_ptr() if c.rows else 16), width
+    d_gate = None if gate is None else call.empty(gate.shape)
+    if gate is not None:
+        c.d_gate, c.d_gate_stride = d_gate.data_ptr(), width
+    vectors = {}
+    for label, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
+                     ("pre_bias", pre_bias)):
+        vectors[label] = None if t is None else call.empty(width)
+        if t is not None:
+            setattr(c, "d_" + label, vectors[label].data_ptr())
+    with call.current():
+        ws = call.workspace(lib.dpc_residual_norm_workspace, ctypes.byref(c))
+        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.dpc_residual_norm_backward(call.stream(), ctypes.byref(c)))
+    return ResidualNormGradients(stream=d_in, branch=d_branch, gate=d_gate, **vectors)
+
+
+# ------------------------------------------------------------------------------ packed activations
+def _activation(name, activation):
+    key = activation.to_string() if isinstance(activation, Activation) else activation
+    if key not in ACT_IDS:
+        raise ValueError(f"{name}: activation {activation!r} is none of {sorted(ACT_IDS)}")
+    return ACT_IDS[key]
+
+
+class PackedActivations:
+    """A tensor [..., width] in 8 bits: ``codes`` (int8, its shape) and ``scales`` (float32 [..., ceil(width / 128)]);
+    the value of an element is its code times its block's scale."""
+
+    def __init__(self, codes, scales):
+        torch = _torch()
+        if not torch.is_tensor(codes) or codes.dtype != torch.int8 or codes.dim() < 2 or not codes.is_contiguous():
+            raise ValueError("PackedActivations: codes has to be a contiguous int8 tensor [..., width]")
+        shape = (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK))
+        if not torch.is_tensor(scales) or scales.dtype != torch.float32 or tuple(scales.shape) != shape or \
+                not scales.is_contiguous() or scales.device != codes.device:
+            raise ValueError(f"PackedActivations: scales has to be a contiguous float32 tensor {shape} beside the codes")
+        self.codes, self.scales = codes, scales
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    def unpack(self, dtype=None):
+        """The values, in ``dtype`` (float32 or bfloat16; default float32)."""
+        torch = _torch()
+        out = torch.empty(self.shape, dtype=dtype or torch.float32, device=self.codes.device)
+        call = _Call("PackedActivations.unpack", "the result", out)
+        _packed_backward(call, self, ACT_IDS["linear"], None, None, out)
+        return out
+
+
+def _packed_backward(call, packed, act, d_out, d_preact, out):
+    lib = _lib.load()
+    width = packed.shape[-1]
+    rows = math.prod(packed.shape[:-1])
+    stride = 0 if d_out is None else call.matrix("d_out", d_out, packed.shape)[2]
+    with call.current():
+        _lib.check(lib.dpc_packed_activation_backward(
+            call.stream(), call.type, act, rows, width, packed.codes.data_ptr(), packed.scales.data_ptr(),
+            None if d_out is None else d_out.data_ptr(), stride, None if d_preact is None else d_preact.data_ptr(), width,
+            None if out is None else out.data_ptr(), width))
+
+
+def activate_and_pack(preact, activation):
+    """``(f(preact), packed)``: a layer's activation (a name such as "gelu", or an ``Activation``), with the
+    pre-activation [..., width] kept in 8 bits for ``packed_activation_backward``.  Every 128 neighbours of the last dimension share
+    a scale, so an element is off by 1/254 of its block's largest at most; a block with an infinity or a NaN becomes NaN."""
+    call = _Call("activate_and_pack", "preact", preact)
+    act = _activation(call.name, activation)
+    rows, width, stride = call.matrix("preact", preact)
+    if width < 1:
+        raise ValueError(f"{call.name}: preact has no columns")
+    lib = _lib.load()
+    out = call.empty(preact.shape)
+    codes = call.empty(preact.shape, dtype=call.torch.int8)
+    scales = call.empty(*preact.shape[:-1], -(-width // BLOCK), dtype=call.torch.float32)
+    with call.current():
+        _lib.check(lib.dpc_activate_and_pack(call.stream(), call.type, act, rows, width, preact.data_ptr(), stride,
+                                             out.data_ptr(), width, codes.data_ptr(), scales.data_ptr()))
+    return out, PackedActivations(codes, scales)
+
+
+def packed_activation_backward(d_out, packed, activation, *, recompute: bool = False):
+    """``(d_preact, out)`` from the gradient of the activation's output: ``d_out * f'(x)`` at the kept x and, with
+    ``recompute``, ``f(x)`` again (else None), which the next layer's weight gradient reads."""
+    call = _Call("packed_activation_backward", "d_out", d_out)
+    act = _activation(call.name, activation)
+    if not isinstance(packed, PackedActivations):
+        raise TypeError(f"{call.name}: packed is a {type(packed).__name__}, not PackedActivations")
+    call.tensor("packed", packed.codes, call.torch.int8)
+    d_preact = call.empty(packed.shape)
+    out = call.empty(packed.shape) if recompute else None
+    _packed_backward(call, packed, act, d_out, d_preact, out)
+    return d_preact, out

@@ -628,6 +628,115 @@ DPC_API dpc_ctx* dpcn_conv_context(dpcn_conv_net* net);
 DPC_API dpc_conv_plan* dpcn_conv_plan(dpcn_conv_net* net);
 DPC_API int64_t dpcn_conv_launch_count(dpcn_conv_net* net);
 
+/* ------------------------------------------------------------------------------------
+ * Operators of deep stacks with large outputs, beside the layers above: the loss over a large
+ * vocabulary with its gradient, the norms around a residual block with their gradients, and
+ * activations kept in 8 bits for the backward pass.  They work on DEVICE pointers of the caller, on
+ * `stream` (a cudaStream_t; NULL: the default stream) of the device that is current on the calling
+ * thread.  Nothing is allocated and nothing waits for the GPU, so every call can be captured into a
+ * CUDA graph; what they need beside their tensors is the caller's workspace (device memory on a
+ * 256-byte boundary, of the size that the *_workspace function tells for the same description, free
+ * again when the call's work is done: calls that may overlap on the GPU have a workspace each).  All tensors of a call have the one
+ * type; matrices are row-major with unit stride along a row and a stride in ELEMENTS between rows.  Outputs overlap neither
+ * inputs nor one another.  Sums, softmax and norm statistics are 32-bit; an output is rounded once.  The same call on the
+ * same inputs gives the same bits.
+ * ---------------------------------------------------------------------------------- */
+typedef enum dpc_type
+{
+  DPC_TYPE_F32 = 0,
+  DPC_TYPE_BF16 = 1
+} dpc_type;
+
+/* Softmax cross entropy of rows of hidden [rows, width] against a vocabulary weight [vocab, width]:
+ *   l = scale * hidden . weight^T + bias     lse = log sum_v exp l     loss = lse - l[target]
+ * The logits are never kept.  A row whose target is ignore_index or lies outside [0, vocab) is ignored: its loss and
+ * lse are 0, its gradient is 0, and what it holds (infinities and NaN too) reaches nothing.
+ * Backward, from the forward call's lse and g = dL/dloss (grad_loss, grad_stride 1; or one value for all rows,
+ * grad_stride 0):  s = g (softmax(l) - onehot);  d_hidden = scale s weight,  d_weight = scale s^T hidden,
+ * d_bias = sum of s over the rows.  f32 tensors are multiplied to 32 bits (three bf16 planes each, six
+ * products); with bf16 tensors s is rounded to bf16 before its two products.  rows may be 0 (d_weight and
+ * d_bias are then zeros); rows, width, vocab and strides 2^28 at most.  A device-side wait that gave up (about 2 s) leaves
+ * NaN in loss, lse, d_hidden and d_bias; d_weight is then undefined. */
+typedef struct dpc_vocab_ce
+{
+  int64_t rows, width, vocab;
+  int64_t hidden_stride, weight_stride;
+  int32_t type;           /* dpc_type */
+  float scale;            /* positive */
+  int64_t ignore_index;
+  const void *hidden, *weight;
+  const void* bias;       /* [vocab] or NULL */
+  const int64_t* targets; /* [rows] */
+  float *loss, *lse;      /* [rows]; backward reads lse and leaves loss alone */
+  /* backward only */
+  const float* grad_loss;
+  int64_t grad_stride;
+  void *d_hidden, *d_weight;
+  int64_t d_hidden_stride, d_weight_stride;
+  void* d_bias; /* or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} dpc_vocab_ce;
+/* Pointers of the description have to be those of the call: an operand off a 16-byte boundary is copied. */
+DPC_API int dpc_vocab_ce_workspace(const dpc_vocab_ce* call, int backward, size_t* bytes);
+DPC_API int dpc_vocab_ce_forward(void* stream, const dpc_vocab_ce* call);
+DPC_API int dpc_vocab_ce_backward(void* stream, const dpc_vocab_ce* call);
+
+/* The end of one residual block and the start of the next, in one pass over the rows:
+ *   u = post_norm ? norm(branch) * post_weight + post_bias : branch
+ *   new_stream = stream_scale * stream + branch_scale * gate * u
+ *   normed = norm(new_stream) * pre_weight + pre_bias
+ * norm(v) = (v - mean) / sqrt(mean of (v - mean)^2 + eps) over a row, with mean = 0 for DPC_NORM_RMS.  Weights,
+ * biases and the gate may be NULL (ones, zeros, ones).  gate [groups, width]: row n takes the gate of group
+ * n / (rows / groups); groups divides rows.  branch NULL (before the first block): new_stream = stream, which is
+ * not written; stream_scale is then 1 and there is no gate and no post norm.
+ * stats [rows, 4]: mean and 1/deviation of the branch (0, 0 without post_norm), of the new stream (before it is rounded).
+ * Backward reads new_stream, branch and stats: d_normed and d_new_stream (NULL: none) are the gradients
+ * of the two outputs; d_branch, d_gate and the gradients of weights and biases are written where the
+ * tensor is given (a gradient pointer may be NULL: not wanted).  width 16384 at most; rows may be 0 (vector gradients are
+ * then zeros). */
+typedef enum dpc_norm
+{
+  DPC_NORM_RMS = 0,
+  DPC_NORM_LAYER = 1
+} dpc_norm;
+typedef struct dpc_residual_norm
+{
+  int64_t rows, width, groups;
+  int32_t type, norm, post_norm; /* dpc_type, dpc_norm, 0 or 1 */
+  float stream_scale, branch_scale, eps;
+  const void *stream, *branch, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+  int64_t stream_stride, branch_stride, gate_stride;
+  void *new_stream, *normed; /* backward reads new_stream */
+  int64_t new_stream_stride, normed_stride;
+  float* stats;
+  /* backward only */
+  const void *d_normed, *d_new_stream;
+  int64_t d_normed_stride, d_new_stream_stride;
+  void *d_stream, *d_branch, *d_gate;
+  int64_t d_stream_stride, d_branch_stride, d_gate_stride;
+  void *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
+  void* workspace;
+  size_t workspace_bytes;
+} dpc_residual_norm;
+DPC_API int dpc_residual_norm_forward(void* stream, const dpc_residual_norm* call);
+DPC_API int dpc_residual_norm_workspace(const dpc_residual_norm* call, size_t* bytes); /* of backward */
+DPC_API int dpc_residual_norm_backward(void* stream, const dpc_residual_norm* call);
+
+/* out = f(x), with x kept in 8 bits: every 128 elements of a row (the last block may be shorter) share
+ * scales[row, block] = max|x| / 127, codes[row, col] = round(x * (127 / max|x|)), ties to even; x is then code * scale.  A
+ * block with nothing of 2^-100 or larger is held as zeros; one with an infinity or a NaN has a NaN as its scale
+ * (and gradient).  codes [rows, width] and scales [rows, ceil(width / 128)] have no gaps; out NULL: not
+ * wanted. */
+DPC_API int dpc_activate_and_pack(void* stream, int type, int act, int64_t rows, int64_t width, const void* x,
+                                  int64_t x_stride, void* out, int64_t out_stride, int8_t* codes, float* scales);
+/* d_preact = d_out * f'(x) and out = f(x) from the packed x; out NULL: not wanted; d_out and d_preact NULL: only out
+ * (with DPC_ACT_LINEAR the kept values themselves). */
+DPC_API int dpc_packed_activation_backward(void* stream, int type, int act, int64_t rows, int64_t width,
+                                           const int8_t* codes, const float* scales, const void* d_out,
+                                           int64_t d_out_stride, void* d_preact, int64_t d_preact_stride, void* out,
+                                           int64_t out_stride);
+
 #ifdef __cplusplus
 }
 #endif
