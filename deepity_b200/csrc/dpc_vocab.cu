@@ -3,8 +3,8 @@
 //
 //   l[n,v] = scale * sum_k hidden[n,k] weight[v,k] + bias[v]
 //   lse[n] = log sum_v exp l[n,v]          loss[n] = lse[n] - l[n, target[n]]
-//   s[n,v] = scale * g[n] * (exp(l[n,v] - lse[n]) - [v == target[n]])         g = dL/dloss
-//   d_hidden = s weight      d_weight = s^T hidden      d_bias = sum_n s / scale
+//   s[n,v] = g[n] / G * (exp(l[n,v] - lse[n]) - [v == target[n]])       g = dL/dloss, G = max |g|
+//   d_hidden = scale G s weight      d_weight = scale G s^T hidden      d_bias = G sum_n s
 //
 // Forward: one product whose epilogue keeps, of every 128 columns, the maximum and the sum of the
 // exponentials of a row (8 bytes instead of 128 logits), then a kernel that joins them.  Backward, for
@@ -13,15 +13,20 @@
 // recomputed product is a quarter of the arithmetic; keeping the logits of 8192 rows x 128000 words in 32
 // bits instead would be 4.2 GB.
 //
-// One persistent kernel does all four products: 256 x 256 tiles on CTA pairs (cta_group::2), 64-deep
+// One persistent kernel does all four products: 256-row tiles on CTA pairs (cta_group::2), 64-deep
 // stages filled by TMA, accumulators double-buffered in tensor memory so that the epilogue warps work
 // on a tile while the next one is multiplied.  A row of the vocabulary or a batch of any length is a tile
 // whose outside TMA fills with zeros.
 //
+// bf16 tensors: tiles 256 wide.  s is rounded to bf16 (half a step, 2^-8, of each of its values): the tensor
+// cores take no wider operand beside bf16 weights, and the sums over it are in 32 bits and are rounded
+// to bf16 themselves.
+//
 // 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low) in the six products
-// whose terms reach 2^-24, smallest first; s is held in as many planes.  For bf16 tensors s is rounded to
-// bf16 (half a step, 2^-9, of each of its values): the tensor cores take no wider operand beside bf16
-// weights, and the sums over it are in 32 bits and are rounded to bf16 themselves.
+// whose terms reach 2^-24, smallest first; s is held in as many planes.  The tensor cores truncate their 32-bit sums,
+// which over the 628 additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm); so a contraction is
+// cut into runs of 8 stages (32 additions) whose sums the epilogue warps add up in registers, rounded to
+// nearest.  They have registers for tiles 128 wide.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -40,16 +45,25 @@ namespace
 using namespace dpc::ptx;
 using namespace dpc::ops;
 
-constexpr int kTile = 256;       // rows and columns of a pair's tile
-constexpr int kRows = 128;       // rows of A, and of B, that one CTA holds
+constexpr int kTile = 256;       // rows of a pair's tile, and columns but for 32-bit tensors
+constexpr int kRows = 128;       // rows of A that one CTA holds
 constexpr int kDepth = 64;       // contraction depth of a stage: 128 bytes, one swizzle row
-constexpr int kStages = 6;
-constexpr int kOperandBytes = kRows * kDepth * 2;
-constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kRowBytes = kDepth * 2;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
-constexpr int kTmemColumns = 512;
+constexpr int kRun = 8; // stages whose products the tensor cores add up, where the epilogue warps add the rest
+
+// Tiles of COLS columns: each CTA of a pair holds half of B's rows.
+template <int COLS>
+struct Tile
+{
+  static constexpr int kABytes = kRows * kRowBytes, kBBytes = COLS / 2 * kRowBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 196608 / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+  static constexpr bool kRuns = COLS < kTile;
+  static constexpr int kShare = COLS / 2; // columns of an epilogue warp
+};
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Bytes of slope, and of weight planes, that a piece of the vocabulary may take.
@@ -57,7 +71,7 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;
 
 enum Epilogue
 {
-  EPI_LSE,   // maximum and sum of exponentials of 128 columns of a row
+  EPI_LSE,   // maximum and sum of exponentials of half a tile of a row
   EPI_SLOPE, // s of the piece, in bf16 planes
   EPI_SUM,   // 32-bit sums, added to what earlier pieces left
   EPI_OUT    // the product itself, in the type of the tensors
@@ -69,7 +83,6 @@ struct GemmParams
   int splits, kblocks, passes;
   uint32_t plane_a, plane_b; // plane of a pass, 4 bits each
   int64_t m, n;              // rows and columns of the product
-  int* status;
   // logits
   float factor;     // scale * log2(e)
   const void* bias; // of the piece, or NULL
@@ -77,11 +90,12 @@ struct GemmParams
   const int64_t* targets;
   int64_t vocab, first; // first: vocabulary entry of column 0
   int64_t ignore_index;
-  float2* partial; // EPI_LSE: [128-column block of the vocabulary][row]
+  float2* partial; // EPI_LSE: [block of the vocabulary, half a tile wide][row]
   float* picked;   // EPI_LSE: logit of the target, in units of log 2
   const float* lse;
   const float* grad;
   int64_t grad_stride;
+  const float* grad_top; // the largest gradient of a row's loss, which s is in units of
   float scale;
   __nv_bfloat16* slope;
   int64_t slope_ld, slope_plane;
@@ -154,13 +168,16 @@ __device__ __forceinline__ void logits32(const GemmParams& P, int64_t col, float
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN>
+template <int EPI, bool A_MN, bool B_MN, int COLS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     vocab_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const GemmParams P)
 {
+  using C = Tile<COLS>;
+  constexpr int kStages = C::kStages, kStageBytes = C::kStageBytes;
+  constexpr uint32_t kTmemColumns = 2 * COLS;
   constexpr uint32_t kInstr = (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
-                              ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(kTile >> 3) << 17) |
+                              ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(COLS >> 3) << 17) |
                               ((uint32_t)(kTile >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages =
@@ -197,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1)
   {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                 "r"((uint32_t)kTmemColumns)
+                 "r"(kTmemColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -224,7 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int64_t tm, tn;
         locate(P, item, split, tm, tn);
         range_of(P, split, it, it_end);
-        const int m0 = (int)(tm * kTile) + (int)rank * kRows, n0 = (int)(tn * kTile) + (int)rank * kRows;
+        const int m0 = (int)(tm * kTile) + (int)rank * kRows, n0 = (int)(tn * COLS) + (int)rank * (COLS / 2);
         int pass = it / P.kblocks, kb = it - pass * P.kblocks;
         for (; it < it_end; ++it)
         {
@@ -237,20 +254,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_expect_tx(&full[s], 2 * kStageBytes); // both CTAs' copies count on the leader's barrier
           const uint32_t bar = lead_full + (uint32_t)(s * 8);
           uint8_t* a = stages + s * kStageBytes;
-          uint8_t* b = a + kOperandBytes;
+          uint8_t* b = a + C::kABytes;
           const int pa = (P.plane_a >> (4 * pass)) & 15, pb = (P.plane_b >> (4 * pass)) & 15;
           const int k = kb * kDepth;
           if (A_MN)
           {
             tma_load_3d_pair(a, &map_a, bar, m0, k, pa);
-            tma_load_3d_pair(a + kOperandBytes / 2, &map_a, bar, m0 + 64, k, pa);
+            tma_load_3d_pair(a + 64 * kRowBytes, &map_a, bar, m0 + 64, k, pa);
           }
           else
             tma_load_3d_pair(a, &map_a, bar, k, m0, pa);
           if (B_MN)
           {
             tma_load_3d_pair(b, &map_b, bar, n0, k, pb);
-            tma_load_3d_pair(b + kOperandBytes / 2, &map_b, bar, n0 + 64, k, pb);
+            if (COLS == 256)
+              tma_load_3d_pair(b + 64 * kRowBytes, &map_b, bar, n0 + 64, k, pb);
           }
           else
             tma_load_3d_pair(b, &map_b, bar, k, n0, pb);
@@ -277,61 +295,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     {
       // K-major: rows of 128 bytes, 8 to a swizzle atom.  MN-major: blocks of 64 columns (8 KB apart) of
       // 64 k-rows, 8 k-rows to an atom, 16 k-rows to an instruction.
-      const uint64_t da0 = make_desc(smem_u32(stages), A_MN ? kOperandBytes / 2 : 16, 1024, 2);
-      const uint64_t db0 = make_desc(smem_u32(stages) + kOperandBytes, B_MN ? kOperandBytes / 2 : 16, 1024, 2);
+      const uint64_t da0 = make_desc(smem_u32(stages), A_MN ? 64 * kRowBytes : 16, 1024, 2);
+      const uint64_t db0 = make_desc(smem_u32(stages) + C::kABytes, B_MN ? 64 * kRowBytes : 16, 1024, 2);
       constexpr uint32_t adv_a = (A_MN ? 2048 : 32) >> 4, adv_b = (B_MN ? 2048 : 32) >> 4;
       int s = 0, turn = 0;
       uint32_t phase = 0;
       bool alive = true;
-      for (int64_t item = begin; item < P.items && alive; item += step, ++turn)
+      for (int64_t item = begin; item < P.items && alive; item += step)
       {
-        const int acc = turn & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tempty[acc], ((turn >> 1) & 1) ^ 1, abort_flag)))
-          break;
-        tc_fence_after();
-        const uint32_t d = tmem_base + acc * kTile;
         int it, it_end;
         range_of(P, (int)(item / (P.tiles_m * P.tiles_n)), it, it_end);
-        for (uint32_t more = 0; it < it_end; ++it)
+        while (it < it_end && alive)
         {
-          if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[s], phase, abort_flag)))
+          const int run_end = C::kRuns && it + kRun < it_end ? it + kRun : it_end;
+          const int acc = turn & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tempty[acc], ((turn >> 1) & 1) ^ 1, abort_flag)))
           {
             alive = false;
             break;
           }
+          ++turn;
           tc_fence_after();
-          const uint64_t sa = da0 + (uint64_t)(s * (kStageBytes >> 4)), sb = db0 + (uint64_t)(s * (kStageBytes >> 4));
-#pragma unroll
-          for (int ks = 0; ks < kDepth / 16; ++ks)
+          const uint32_t d = tmem_base + acc * COLS;
+          for (uint32_t more = 0; it < run_end; ++it)
           {
-            tc_mma_bf16_pair(d, sa + (uint64_t)(ks * adv_a), sb + (uint64_t)(ks * adv_b), kInstr, more);
-            more = 1;
+            if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[s], phase, abort_flag)))
+            {
+              alive = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t sa = da0 + (uint64_t)(s * (kStageBytes >> 4)), sb = db0 + (uint64_t)(s * (kStageBytes >> 4));
+#pragma unroll
+            for (int ks = 0; ks < kDepth / 16; ++ks)
+            {
+              tc_mma_bf16_pair(d, sa + (uint64_t)(ks * adv_a), sb + (uint64_t)(ks * adv_b), kInstr, more);
+              more = 1;
+            }
+            tc_commit_pair(smem_u32(&empty[s])); // the stage is free in both CTAs
+            tc_commit_pair(peer_empty + (uint32_t)(s * 8));
+            if (++s == kStages)
+              s = 0, phase ^= 1;
           }
-          tc_commit_pair(smem_u32(&empty[s])); // the stage is free in both CTAs
-          tc_commit_pair(peer_empty + (uint32_t)(s * 8));
-          if (++s == kStages)
-            s = 0, phase ^= 1;
-        }
-        if (alive)
-        {
-          tc_commit_pair(smem_u32(&tfull[acc]));
-          tc_commit_pair(peer_tfull + (uint32_t)(acc * 8));
+          if (alive)
+          {
+            tc_commit_pair(smem_u32(&tfull[acc]));
+            tc_commit_pair(peer_tfull + (uint32_t)(acc * 8));
+          }
         }
       }
     }
   }
   else if (warp >= 4)
   {
-    // ---------------------------------------------------------------- epilogue: a row a lane, 128 columns a warp
+    // ---------------------------------------------------------------- epilogue: a row a lane, half a tile's columns a warp
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     int turn = 0;
-    for (int64_t item = begin; item < P.items; item += step, ++turn)
+    bool alive = true; // a wait gave up: everything from then on is NaN
+    for (int64_t item = begin; item < P.items; item += step)
     {
       int split;
       int64_t tm, tn;
       locate(P, item, split, tm, tn);
       const int64_t row = tm * kTile + rank * kRows + quarter * 32 + lane;
-      const int64_t col0 = tn * kTile + half * 128;
+      const int64_t col0 = tn * COLS + half * C::kShare;
       const bool inside = row < P.m;
       int64_t target = -1; // column of the target, outside the tile: not this one
       bool count = false;
@@ -345,22 +372,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (EPI == EPI_SLOPE && count)
         {
           lse2 = P.lse[row] * kLog2e;
-          slope_scale = P.grad[row * P.grad_stride] * P.scale;
+          slope_scale = __fdiv_rn(P.grad[row * P.grad_stride], *P.grad_top);
+        }
+      }
+      int it, it_end;
+      range_of(P, split, it, it_end);
+      float sums[C::kRuns ? C::kShare / 32 : 1][32];
+      const bool several = it + kRun < it_end;
+      if (C::kRuns)
+      {
+        // the runs but the last, which the loop below adds
+        for (bool first = true; alive && it + kRun < it_end; it += kRun, ++turn, first = false)
+        {
+          const int acc = turn & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag)))
+          {
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * COLS + half * C::kShare;
+#pragma unroll
+          for (int c = 0; c < C::kShare / 32; ++c)
+          {
+            float v[32];
+            __syncwarp();
+            tc_ld32(taddr + 32 * c, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              sums[C::kRuns ? c : 0][i] = first ? v[i] : sums[C::kRuns ? c : 0][i] + v[i];
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_cluster(lead_tempty + (uint32_t)(acc * 8));
         }
       }
       const int acc = turn & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag)))
-        break;
+      if (alive)
+        alive = __all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag));
+      ++turn;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTile + half * 128;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * COLS + half * C::kShare;
+      const float out_factor = EPI == EPI_OUT ? *P.grad_top * P.scale : 1.0f;
       float top = -INFINITY, total = 0.0f;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c)
+#pragma unroll(C::kRuns ? C::kShare / 32 : 1)
+      for (int c = 0; c < C::kShare / 32; ++c)
       {
         const int64_t col = col0 + 32 * c;
         float v[32];
         __syncwarp();
-        tc_ld32(taddr + 32 * c, v);
+        tc_ld32(taddr + 32 * c, v); // (a read of whatever is there, after a wait that gave up)
+        if (C::kRuns && several)
+        {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] += sums[C::kRuns ? c : 0][i];
+        }
+        if (!alive)
+        {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = NAN;
+        }
         if (EPI == EPI_LSE)
         {
           logits32(P, col, v);
@@ -438,6 +512,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         else if (inside && col < P.n)
         {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] *= out_factor;
           if (P.out_wide && col + 32 <= P.n)
           {
             if (P.out_f32)
@@ -474,7 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0)
         mbar_arrive_cluster(lead_tempty + (uint32_t)(acc * 8));
       if (EPI == EPI_LSE && inside)
-        P.partial[((P.first + col0) / 128) * P.m + row] = make_float2(top, total);
+        P.partial[((P.first + col0) / C::kShare) * P.m + row] = make_float2(top, total);
     }
   }
 
@@ -482,12 +559,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_fence_before();
   cluster_sync_all(); // neither CTA leaves while the other may still touch its memory
-  if (threadIdx.x == 0 && *abort_flag)
-    atomicExch(P.status, 1);
   if (warp == 1)
   {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemColumns)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns)
                  : "memory");
   }
 }
@@ -497,8 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 __global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restrict__ partial, int64_t parts, int64_t rows,
                                                          int row_shift, const float* __restrict__ picked,
                                                          const int64_t* __restrict__ targets, int64_t vocab,
-                                                         int64_t ignore_index, const int* __restrict__ status,
-                                                         float* __restrict__ loss, float* __restrict__ lse)
+                                                         int64_t ignore_index, float* __restrict__ loss, float* __restrict__ lse)
 {
   __shared__ float tops[256], sums[256];
   const int per = 1 << row_shift, r = threadIdx.x & (per - 1), lanes = 256 >> row_shift;
@@ -528,10 +602,7 @@ __global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restric
   if ((int)threadIdx.x < per && row < rows)
   {
     const bool count = counted(targets[row], vocab, ignore_index);
-    float l = tops[r] + log2f(sums[r]);
-    float d = l - (count ? picked[row] : 0.0f);
-    if (*status) // a device-side wait gave up: the parts are not complete
-      l = d = NAN;
+    const float l = tops[r] + log2f(sums[r]), d = l - (count ? picked[row] : 0.0f);
     lse[row] = count ? l * kLn2 : 0.0f;
     loss[row] = count ? d * kLn2 : 0.0f;
   }
@@ -566,18 +637,53 @@ __global__ void __launch_bounds__(256) vocab_planes_kernel(const T* __restrict__
   }
 }
 
-// out[row][col] = the sum of the splits' sums, in the type of the tensors.
+// The largest |g| of the rows that count: s is held in units of it, so that in a mean over the rows (all g
+// alike) the -1 of a target is exactly -1 in bf16 and not a rounded 1/rows, whose error all rows would share.  1
+// where it is 0 or no number.
+__global__ void __launch_bounds__(1024) vocab_gradient_kernel(const float* __restrict__ grad, int64_t stride,
+                                                              const int64_t* __restrict__ targets, int64_t rows,
+                                                              int64_t vocab, int64_t ignore_index, float* __restrict__ top)
+{
+  __shared__ float tops[32];
+  float most = 0.0f;
+  bool bad = false;
+  for (int64_t row = threadIdx.x; row < rows; row += 1024)
+    if (counted(targets[row], vocab, ignore_index))
+    {
+      const float g = fabsf(grad[row * stride]);
+      most = fmaxf(most, g), bad |= !(g < INFINITY);
+    }
+  if (bad)
+    most = INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if ((threadIdx.x & 31) == 0)
+    tops[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x < 32)
+  {
+    most = tops[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (threadIdx.x == 0)
+      *top = most > 0.0f && most < INFINITY ? most : 1.0f;
+  }
+}
+
+// out[row][col] = factor * the sum of the splits' sums, in the type of the tensors.
 template <typename T>
 __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict__ sum, int64_t ld, int64_t split_stride,
                                                         int splits, int64_t rows, int64_t cols, T* __restrict__ out,
-                                                        int64_t out_ld, const int* __restrict__ status)
+                                                        int64_t out_ld, const float* __restrict__ grad_top, float scale)
 {
-  const float poison = *status ? NAN : 0.0f;
+  const float factor = *grad_top * scale;
   const int64_t chunks = (cols + 3) / 4, total = rows * chunks;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
   {
     const int64_t row = i / chunks, col = (i - row * chunks) * 4;
-    float4 v = make_float4(poison, poison, poison, poison);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s = 0; s < splits; ++s)
     {
       const float4 w = *reinterpret_cast<const float4*>(sum + s * split_stride + row * ld + col);
@@ -587,16 +693,15 @@ __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict_
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (col + k < cols)
-        out[row * out_ld + col + k] = from_float<T>(f[k]);
+        out[row * out_ld + col + k] = from_float<T>(f[k] * factor);
   }
 }
 
-// out[col] = factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
+// out[col] = *factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
                                                             int64_t plane, int planes, int64_t rows, int64_t cols,
-                                                            float factor, T* __restrict__ out,
-                                                            const int* __restrict__ status)
+                                                            const float* __restrict__ factor, T* __restrict__ out)
 {
   __shared__ float2 parts[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -615,11 +720,10 @@ __global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16*
     total = make_float2(0.0f, 0.0f);
     for (int w = 0; w < 8; ++w)
       total.x += parts[w][lane].x, total.y += parts[w][lane].y;
-    const float poison = *status ? NAN : 0.0f;
     if (col < cols)
-      out[col] = from_float<T>(fmaf(total.x, factor, poison));
+      out[col] = from_float<T>(total.x * *factor);
     if (col + 1 < cols)
-      out[col + 1] = from_float<T>(fmaf(total.y, factor, poison));
+      out[col + 1] = from_float<T>(total.y * *factor);
   }
 }
 
@@ -652,17 +756,18 @@ struct Operand
   int64_t cols, rows, ld, plane;
 };
 
-template <int EPI, bool A_MN, bool B_MN>
+template <int EPI, bool A_MN, bool B_MN, int COLS>
 int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, int planes, int64_t m, int64_t n,
             int64_t contraction, GemmParams P)
 {
+  using C = Tile<COLS>;
   CUtensorMap map_a, map_b;
   if (int rc = operand_map(&map_a, a.base, a.cols, a.rows, a.ld, planes, a.plane, A_MN ? kDepth : kRows))
     return rc;
-  if (int rc = operand_map(&map_b, b.base, b.cols, b.rows, b.ld, planes, b.plane, B_MN ? kDepth : kRows))
+  if (int rc = operand_map(&map_b, b.base, b.cols, b.rows, b.ld, planes, b.plane, B_MN ? kDepth : COLS / 2))
     return rc;
   P.m = m, P.n = n;
-  P.tiles_m = ceil_div(m, kTile), P.tiles_n = ceil_div(n, kTile);
+  P.tiles_m = ceil_div(m, kTile), P.tiles_n = ceil_div(n, COLS);
   P.group_m = std::min<int64_t>(P.tiles_m, 32);
   P.kblocks = (int)ceil_div(contraction, kDepth);
   // Plane pairs of a pass, smallest terms first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
@@ -672,21 +777,31 @@ int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, 
   P.splits = (int)std::min<int64_t>(P.splits, (int64_t)P.kblocks * P.passes);
   P.items = P.tiles_m * P.tiles_n * P.splits;
   P.planes = planes;
-  auto kernel = vocab_product_kernel<EPI, A_MN, B_MN>;
-  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  auto kernel = vocab_product_kernel<EPI, A_MN, B_MN, COLS>;
+  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
   const int blocks = 2 * (int)std::min<int64_t>(P.items, pairs);
-  kernel<<<blocks, kThreads, kSmemBytes, stream>>>(map_a, map_b, P);
+  kernel<<<blocks, kThreads, C::kSmemBytes, stream>>>(map_a, map_b, P);
   return launched("vocab_product_kernel");
+}
+
+// Tiles 128 wide, and sums in runs, for 32-bit tensors.
+template <int EPI, bool A_MN, bool B_MN>
+int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, int planes, int64_t m, int64_t n,
+            int64_t contraction, const GemmParams& P)
+{
+  return planes == 3 ? product<EPI, A_MN, B_MN, 128>(stream, pairs, a, b, planes, m, n, contraction, P)
+                     : product<EPI, A_MN, B_MN, 256>(stream, pairs, a, b, planes, m, n, contraction, P);
 }
 
 struct Layout
 {
   int pairs = 0, planes = 1, splits = 1;
   bool copy_hidden = false, copy_weight = false;
+  int64_t share = 0; // columns of a partial sum of exponentials
   int64_t kp = 0;    // columns of the copies
   int64_t ks = 0;    // columns of the sums of d_hidden
   int64_t piece = 0; // vocabulary entries at a time, a multiple of the tile (or all of them)
-  size_t status = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
+  size_t grad_top = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
 };
 
 bool tma_ready(const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
@@ -726,6 +841,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   // does not reach d_weight as 0 * inf)
   L.copy_hidden = backward || L.planes > 1 || !tma_ready(c->hidden, c->hidden_stride);
   L.copy_weight = L.planes > 1 || !tma_ready(c->weight, c->weight_stride);
+  L.share = L.planes == 3 ? Tile<128>::kShare : Tile<256>::kShare;
   L.kp = round_up(c->width, 8);
   L.ks = round_up(c->width, kTile);
   const int64_t all = round_up(c->vocab, kTile);
@@ -744,7 +860,8 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  L.status = take(sizeof(int));
+  if (backward)
+    L.grad_top = take(sizeof(float));
   if (L.copy_hidden)
     L.hidden = take((size_t)c->rows * L.kp * 2 * L.planes);
   if (L.copy_weight)
@@ -752,7 +869,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   if (backward)
   {
     // Few tiles of d_hidden: the contraction over the piece is shared out, 4 blocks of it at least each.
-    const int64_t tiles = ceil_div(c->rows, kTile) * (L.ks / kTile);
+    const int64_t tiles = ceil_div(c->rows, kTile) * (L.ks / (2 * L.share));
     const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth) * (L.planes == 3 ? 6 : 1);
     L.splits = (int)std::max<int64_t>(1, std::min(L.pairs / std::max<int64_t>(1, tiles), blocks / 4));
     L.slope = take((size_t)c->rows * L.piece * 2 * L.planes);
@@ -760,7 +877,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   }
   else
   {
-    L.partial = take((size_t)(all / 128) * c->rows * sizeof(float2));
+    L.partial = take((size_t)(all / L.share) * c->rows * sizeof(float2));
     L.picked = take((size_t)c->rows * sizeof(float));
   }
   L.bytes = at;
@@ -832,7 +949,7 @@ GemmParams base_params(const dpc_vocab_ce* c, const Layout& L, int64_t first, ch
 {
   GemmParams P = {};
   P.splits = 1;
-  P.status = reinterpret_cast<int*>(ws + L.status);
+  P.grad_top = reinterpret_cast<const float*>(ws + L.grad_top);
   P.factor = c->scale * kLog2e;
   P.scale = c->scale;
   P.bias = c->bias ? at_row(c->bias, c->type, first) : nullptr;
@@ -857,7 +974,6 @@ int forward(cudaStream_t stream, const dpc_vocab_ce* c)
   if (int rc = workspace_ok(c, L, who))
     return rc;
   char* ws = static_cast<char*>(c->workspace);
-  DPC_CUDA(cudaMemsetAsync(ws + L.status, 0, sizeof(int), stream));
   Operand hidden, weight;
   if (int rc = prepare_hidden(stream, c, L, false, ws, hidden))
     return rc;
@@ -876,9 +992,9 @@ int forward(cudaStream_t stream, const dpc_vocab_ce* c)
   while (row_shift < 5 && ((int64_t)1 << row_shift) < c->rows)
     ++row_shift;
   vocab_join_kernel<<<(unsigned)ceil_div(c->rows, (int64_t)1 << row_shift), 256, 0, stream>>>(
-      reinterpret_cast<const float2*>(ws + L.partial), round_up(c->vocab, kTile) / 128, c->rows, row_shift,
+      reinterpret_cast<const float2*>(ws + L.partial), round_up(c->vocab, L.planes == 3 ? 128 : kTile) / L.share, c->rows, row_shift,
       reinterpret_cast<const float*>(ws + L.picked), c->targets, c->vocab, c->ignore_index,
-      reinterpret_cast<const int*>(ws + L.status), c->loss, c->lse);
+      c->loss, c->lse);
   return launched("vocab_join_kernel");
 }
 
@@ -911,10 +1027,13 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
   if (int rc = workspace_ok(c, L, who))
     return rc;
   char* ws = static_cast<char*>(c->workspace);
-  int* status = reinterpret_cast<int*>(ws + L.status);
+  float* grad_top = reinterpret_cast<float*>(ws + L.grad_top);
   float* sum = reinterpret_cast<float*>(ws + L.sum);
   __nv_bfloat16* slope = reinterpret_cast<__nv_bfloat16*>(ws + L.slope);
-  DPC_CUDA(cudaMemsetAsync(status, 0, sizeof(int), stream));
+  vocab_gradient_kernel<<<1, 1024, 0, stream>>>(c->grad_loss, c->grad_stride, c->targets, c->rows, c->vocab,
+                                                c->ignore_index, grad_top);
+  if (int rc = launched("vocab_gradient_kernel"))
+    return rc;
   Operand hidden, weight;
   if (int rc = prepare_hidden(stream, c, L, true, ws, hidden))
     return rc;
@@ -946,12 +1065,10 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
       const unsigned blocks = (unsigned)ceil_div(count, 64);
       if (c->type == DPC_TYPE_F32)
         vocab_columns_kernel<float><<<blocks, 256, 0, stream>>>(slope, L.piece, plane, L.planes, c->rows, count,
-                                                                1.0f / c->scale, static_cast<float*>(c->d_bias) + first,
-                                                                status);
+                                                                grad_top, static_cast<float*>(c->d_bias) + first);
       else
         vocab_columns_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(
-            slope, L.piece, plane, L.planes, c->rows, count, 1.0f / c->scale,
-            static_cast<__nv_bfloat16*>(c->d_bias) + first, status);
+            slope, L.piece, plane, L.planes, c->rows, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
       if (int rc = launched("vocab_columns_kernel"))
         return rc;
     }
@@ -959,11 +1076,11 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
   const int blocks = grid_for(c->rows * ceil_div(c->width, 4));
   if (c->type == DPC_TYPE_F32)
     vocab_sum_kernel<float><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
-                                                        static_cast<float*>(c->d_hidden), c->d_hidden_stride, status);
+                                                        static_cast<float*>(c->d_hidden), c->d_hidden_stride, grad_top, c->scale);
   else
     vocab_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
                                                                 static_cast<__nv_bfloat16*>(c->d_hidden),
-                                                                c->d_hidden_stride, status);
+                                                                c->d_hidden_stride, grad_top, c->scale);
   return launched("vocab_sum_kernel");
 }
 } // namespace

@@ -31,25 +31,36 @@ def _torch():
     return torch
 
 
+def _stream(torch, device):
+    """The handle of torch's current stream; without the Stream object around it where torch offers that (7 us less)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 class _Call:
-    """What the tensors of one call have in common: type and device, taken from the first."""
+    """What the tensors of one call have in common: type and device, taken from the first.  (Few and cheap
+    steps: a call for one token is bound by the host.)"""
+    __slots__ = ("torch", "name", "dtype", "device", "type")
 
     def __init__(self, name, first_name, first):
-        torch = _torch()
-        self.torch, self.name = torch, name
-        if not torch.is_tensor(first):
+        torch = self.torch = _torch()
+        self.name = name
+        if not isinstance(first, torch.Tensor):
             raise TypeError(f"{name}: {first_name} has to be a torch tensor, not {type(first).__name__}")
-        if first.dtype not in (torch.float32, torch.bfloat16):
+        self.dtype, self.device = first.dtype, first.device
+        if self.dtype is torch.bfloat16:
+            self.type = 1
+        elif self.dtype is torch.float32:
+            self.type = 0
+        else:
             raise TypeError(f"{name}: {first_name} is {first.dtype}; float32 and bfloat16 are supported")
         if not first.is_cuda:
             raise ValueError(f"{name}: {first_name} is on {first.device}; there is no CPU path")
-        self.dtype, self.device = first.dtype, first.device
-        self.type = 0 if first.dtype == torch.float32 else 1
 
     def tensor(self, label, t, dtype=None):
-        if not self.torch.is_tensor(t):
+        if not isinstance(t, self.torch.Tensor):
             raise TypeError(f"{self.name}: {label} has to be a torch tensor, not {type(t).__name__}")
-        if t.dtype != (dtype or self.dtype):
+        if t.dtype is not (dtype or self.dtype):
             raise TypeError(f"{self.name}: {label} is {t.dtype}, {dtype or self.dtype} is needed")
         if t.device != self.device:
             raise ValueError(f"{self.name}: {label} is on {t.device}, the call on {self.device}")
@@ -57,12 +68,15 @@ class _Call:
 
     def matrix(self, label, t, shape=None):
         """(rows, width, row stride) of a tensor whose leading dimensions one stride describes."""
-        t = self.tensor(label, t)
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{self.name}: {label} is {tuple(t.shape)}, {tuple(shape)} is needed")
-        if t.dim() < 2:
+        found = self.tensor(label, t).shape
+        if shape is not None and found != shape:
+            raise ValueError(f"{self.name}: {label} is {tuple(found)}, {tuple(shape)} is needed")
+        if len(found) < 2:
             raise ValueError(f"{self.name}: {label} needs two dimensions at least, it has {t.dim()}")
-        rows, width = math.prod(t.shape[:-1]), t.shape[-1]
+        width = found[-1]
+        rows = found[0] if len(found) == 2 else math.prod(found[:-1])
+        if t.is_contiguous():
+            return rows, width, max(width, 1)
         if width > 1 and t.stride(-1) != 1:
             raise ValueError(f"{self.name}: the last dimension of {label} has to be contiguous")
         try:
@@ -74,23 +88,28 @@ class _Call:
     def vector(self, label, t, width):
         if t is None:
             return None
-        if tuple(self.tensor(label, t).shape) != (width,) or (width > 1 and t.stride(0) != 1):
+        if self.tensor(label, t).shape != (width,) or not t.is_contiguous():
             raise ValueError(f"{self.name}: {label} has to be a contiguous vector of {width}")
         return t.data_ptr()
 
-    def empty(self, *shape, dtype=None):
-        return self.torch.empty(*shape, dtype=dtype or self.dtype, device=self.device)
+    def empty(self, shape, dtype=None):
+        return self.torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
 
-    def workspace(self, size_of, *args):
-        size = ctypes.c_size_t()
-        _lib.check(size_of(*args, ctypes.byref(size)))
-        return self.empty(size.value, dtype=self.torch.uint8)
-
-    def current(self):
-        return self.torch.cuda.device(self.device)
-
-    def stream(self):
-        return self.torch.cuda.current_stream(self.device).cuda_stream
+    def run(self, function, *args, workspace=None, call=None):
+        """function(stream, *args) on torch's current stream of the tensors' device; ``workspace(call, size)`` tells
+        first how much the call needs."""
+        cuda = self.torch.cuda
+        if cuda.current_device() != self.device.index:
+            with cuda.device(self.device):
+                return self.run(function, *args, workspace=workspace, call=call)
+        if call is not None:
+            if workspace is not None:
+                size = ctypes.c_size_t()
+                _lib.check(workspace(size))
+                held = self.empty(size.value, self.torch.uint8)  # (its memory is reused in stream order)
+                call.workspace, call.workspace_bytes = held.data_ptr(), size.value
+            args = (ctypes.byref(call),)
+        _lib.check(function(_stream(self.torch, self.device), *args))
 
 
 # ------------------------------------------------------------------------------ vocabulary loss
@@ -101,12 +120,11 @@ class VocabGradients(NamedTuple):
 
 
 def _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index):
-    torch = call.torch
     rows, width, hidden_stride = call.matrix("hidden", hidden)
-    if call.tensor("weight", weight).dim() != 2 or weight.shape[1] != width:
+    vocab, weight_width, weight_stride = call.matrix("weight", weight)
+    if weight.dim() != 2 or weight_width != width:
         raise ValueError(f"{call.name}: weight is {tuple(weight.shape)}, (vocabulary, {width}) is needed")
-    vocab, _, weight_stride = call.matrix("weight", weight)
-    if call.tensor("targets", targets, torch.int64).shape != hidden.shape[:-1]:
+    if call.tensor("targets", targets, call.torch.int64).shape != hidden.shape[:-1]:
         raise ValueError(f"{call.name}: targets is {tuple(targets.shape)}, {tuple(hidden.shape[:-1])} is needed")
     targets = targets.contiguous()
     c = _lib.VocabCe(rows=rows, width=width, vocab=vocab, hidden_stride=hidden_stride, weight_stride=weight_stride,
@@ -125,13 +143,11 @@ def vocab_cross_entropy(hidden, weight, targets, bias=None, *, scale: float = 1.
     call = _Call("vocab_cross_entropy", "hidden", hidden)
     c, targets = _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index)
     lib = _lib.load()
-    loss = call.empty(targets.shape, dtype=call.torch.float32)
-    lse = call.empty(targets.shape, dtype=call.torch.float32)
+    loss = call.empty(targets.shape, call.torch.float32)
+    lse = call.empty(targets.shape, call.torch.float32)
     c.loss, c.lse = loss.data_ptr(), lse.data_ptr()
-    with call.current():
-        ws = call.workspace(lib.dpc_vocab_ce_workspace, ctypes.byref(c), 0)
-        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.check(lib.dpc_vocab_ce_forward(call.stream(), ctypes.byref(c)))
+    call.run(lib.dpc_vocab_ce_forward, call=c,
+             workspace=lambda size: lib.dpc_vocab_ce_workspace(ctypes.byref(c), 0, ctypes.byref(size)))
     return loss, lse
 
 
@@ -157,10 +173,8 @@ def vocab_cross_entropy_backward(grad_loss, hidden, weight, targets, lse, bias=N
     c.d_hidden, c.d_hidden_stride = d_hidden.data_ptr(), c.width
     c.d_weight, c.d_weight_stride = d_weight.data_ptr(), c.width
     c.d_bias = None if bias is None else d_bias.data_ptr()
-    with call.current():
-        ws = call.workspace(lib.dpc_vocab_ce_workspace, ctypes.byref(c), 1)
-        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.check(lib.dpc_vocab_ce_backward(call.stream(), ctypes.byref(c)))
+    call.run(lib.dpc_vocab_ce_backward, call=c,
+             workspace=lambda size: lib.dpc_vocab_ce_workspace(ctypes.byref(c), 1, ctypes.byref(size)))
     return VocabGradients(d_hidden, d_weight, d_bias)
 
 
@@ -179,14 +193,15 @@ def _norm_call(call, like, branch, norm, post_norm, post_weight, post_bias, gate
                pre_weight, pre_bias, eps):
     if norm not in _NORMS:
         raise ValueError(f"{call.name}: norm {norm!r} is none of {sorted(_NORMS)}")
-    rows, width, _ = call.matrix("the residual stream", like)
+    rows, width, stride = call.matrix("the residual stream", like)
     post_norm = post_weight is not None or post_bias is not None if post_norm is None else bool(post_norm)
     c = _lib.ResidualNorm(rows=rows, width=width, groups=1, type=call.type, norm=_NORMS[norm], post_norm=post_norm,
                           stream_scale=stream_scale, branch_scale=branch_scale, eps=eps,
                           post_weight=call.vector("post_weight", post_weight, width),
                           post_bias=call.vector("post_bias", post_bias, width),
                           pre_weight=call.vector("pre_weight", pre_weight, width),
-                          pre_bias=call.vector("pre_bias", pre_bias, width))
+                          pre_bias=call.vector("pre_bias", pre_bias, width), stream_stride=stride,
+                          new_stream_stride=stride)
     if branch is not None:
         c.branch_stride = call.matrix("branch", branch, like.shape)[2]
         c.branch = branch.data_ptr()
@@ -224,15 +239,14 @@ def residual_norm(stream, branch=None, *, norm: str = "rms", post_norm: Optional
     c = _norm_call(call, stream, branch, norm, post_norm, post_weight, post_bias, gate, stream_scale, branch_scale,
                    pre_weight, pre_bias, eps)
     lib = _lib.load()
-    c.stream, c.stream_stride = stream.data_ptr(), call.matrix("stream", stream)[2]
+    c.stream = stream.data_ptr()
     new_stream = stream if branch is None else call.empty(stream.shape)
     normed = call.empty(stream.shape)
-    stats = call.empty(*stream.shape[:-1], 4, dtype=call.torch.float32)
+    stats = call.empty((*stream.shape[:-1], 4), call.torch.float32)
     if branch is not None:
         c.new_stream, c.new_stream_stride = new_stream.data_ptr(), c.width
     c.normed, c.normed_stride, c.stats = normed.data_ptr(), c.width, stats.data_ptr()
-    with call.current():
-        _lib.check(lib.dpc_residual_norm_forward(call.stream(), ctypes.byref(c)))
+    call.run(lib.dpc_residual_norm_forward, call=c)
     return new_stream, normed, stats
 
 
@@ -246,7 +260,7 @@ def residual_norm_backward(d_normed, d_stream, new_stream, branch, stats, *, nor
     c = _norm_call(call, new_stream, branch, norm, post_norm, post_weight, post_bias, gate, stream_scale, branch_scale,
                    pre_weight, pre_bias, 0.0)
     lib, shape, width = _lib.load(), new_stream.shape, c.width
-    c.new_stream, c.new_stream_stride = new_stream.data_ptr(), call.matrix("new_stream", new_stream)[2]
+    c.new_stream = new_stream.data_ptr()
     c.d_normed_stride = call.matrix("d_normed", d_normed, shape)[2]
     c.d_normed = d_normed.data_ptr()
     if d_stream is not None:
@@ -269,10 +283,8 @@ def residual_norm_backward(d_normed, d_stream, new_stream, branch, stats, *, nor
         vectors[label] = None if t is None else call.empty(width)
         if t is not None:
             setattr(c, "d_" + label, vectors[label].data_ptr())
-    with call.current():
-        ws = call.workspace(lib.dpc_residual_norm_workspace, ctypes.byref(c))
-        c.workspace, c.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.check(lib.dpc_residual_norm_backward(call.stream(), ctypes.byref(c)))
+    call.run(lib.dpc_residual_norm_backward, call=c,
+             workspace=lambda size: lib.dpc_residual_norm_workspace(ctypes.byref(c), ctypes.byref(size)))
     return ResidualNormGradients(stream=d_in, branch=d_branch, gate=d_gate, **vectors)
 
 
@@ -316,11 +328,9 @@ def _packed_backward(call, packed, act, d_out, d_preact, out):
     width = packed.shape[-1]
     rows = math.prod(packed.shape[:-1])
     stride = 0 if d_out is None else call.matrix("d_out", d_out, packed.shape)[2]
-    with call.current():
-        _lib.check(lib.dpc_packed_activation_backward(
-            call.stream(), call.type, act, rows, width, packed.codes.data_ptr(), packed.scales.data_ptr(),
-            None if d_out is None else d_out.data_ptr(), stride, None if d_preact is None else d_preact.data_ptr(), width,
-            None if out is None else out.data_ptr(), width))
+    call.run(lib.dpc_packed_activation_backward, call.type, act, rows, width, packed.codes.data_ptr(),
+             packed.scales.data_ptr(), None if d_out is None else d_out.data_ptr(), stride,
+             None if d_preact is None else d_preact.data_ptr(), width, None if out is None else out.data_ptr(), width)
 
 
 def activate_and_pack(preact, activation):
@@ -334,11 +344,10 @@ def activate_and_pack(preact, activation):
         raise ValueError(f"{call.name}: preact has no columns")
     lib = _lib.load()
     out = call.empty(preact.shape)
-    codes = call.empty(preact.shape, dtype=call.torch.int8)
-    scales = call.empty(*preact.shape[:-1], -(-width // BLOCK), dtype=call.torch.float32)
-    with call.current():
-        _lib.check(lib.dpc_activate_and_pack(call.stream(), call.type, act, rows, width, preact.data_ptr(), stride,
-                                             out.data_ptr(), width, codes.data_ptr(), scales.data_ptr()))
+    codes = call.empty(preact.shape, call.torch.int8)
+    scales = call.empty((*preact.shape[:-1], -(-width // BLOCK)), call.torch.float32)
+    call.run(lib.dpc_activate_and_pack, call.type, act, rows, width, preact.data_ptr(), stride, out.data_ptr(), width,
+             codes.data_ptr(), scales.data_ptr())
     return out, PackedActivations(codes, scales)
 
 

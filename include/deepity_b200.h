@@ -656,7 +656,7 @@ typedef enum dpc_type
  * d_bias = sum of s over the rows.  f32 tensors are multiplied to 32 bits (three bf16 planes each, six
  * products); with bf16 tensors s is rounded to bf16 before its two products.  rows may be 0 (d_weight and
  * d_bias are then zeros); rows, width, vocab and strides 2^28 at most.  A device-side wait that gave up (about 2 s) leaves
- * NaN in loss, lse, d_hidden and d_bias; d_weight is then undefined. */
+ * NaN in the results that were not computed. */
 typedef struct dpc_vocab_ce
 {
   int64_t rows, width, vocab;
