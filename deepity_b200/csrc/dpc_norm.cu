@@ -14,6 +14,13 @@
 // squares of what is left), which loses nothing where the mean is large.  Sums over rows (weights,
 // biases, gates) stay in registers while a unit of threads walks its rows, are written once per unit and
 // added by a second kernel in a fixed order: no atomics, the same bits every time.
+//
+// Those sums leave registers for 512 threads an SM, too few to cover the memory's latency with loads of their
+// own: backward fetches its four rows two and more ahead into shared memory by bulk copies.  16384 x 4096 bf16 (805 MB,
+// 123 us at the rate of a copy): 256 us with loads in the threads themselves, 219 with the copies, 168 with arithmetic
+// on pairs and no register spilled; what is left waits for the row's two sums and for weights from L1.  Spills decide
+// here: 100 bytes of them cost 50 us, a second row at once or a warp that only fetches cost more than they gave.
+// Forward: 50 us at 16384 x 2048 bf16 (268 MB, 41 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -23,6 +30,7 @@
 
 #include "dpc_internal.h"
 #include "dpc_operators.cuh"
+#include "dpc_tcgen05.cuh"
 
 namespace
 {
@@ -32,7 +40,8 @@ constexpr int64_t kMaxWidth = 16384;
 
 struct NormParams
 {
-  int64_t rows, width, rows_per_group;
+  int64_t rows, width;
+  int rows_per_group;
   int layer, post, has_branch;
   float a, b, eps, inv_width;
   const void *x, *y, *gate, *wp, *bp, *wn, *bn;
@@ -44,8 +53,9 @@ struct NormParams
   int64_t dh_ld, dr_ld;
   void *dx, *dy, *dg;
   int64_t dx_ld, dy_ld, dg_ld;
-  int64_t units, chunks, chunks_per_group, rows_per_chunk;
-  float *sums, *gate_sums; // [4][units][width], [chunks][width]
+  int units, chunks, chunks_per_group, rows_per_chunk;
+  float *sums, *gate_sums; // [4][units][sums_ld], [chunks][sums_ld]
+  int64_t sums_ld;         // the width, up to a multiple of 8
 };
 
 // The elements of a row that a thread holds, VPT * 8 of them.  WIDE: vectors of 8 neighbours, 16-byte
@@ -114,20 +124,23 @@ __device__ __forceinline__ void store_row(void* base, int64_t offset, int width,
   }
 }
 
-// Two sums over the threads of a row, to all of them.  More than a warp: through one of two buffers in turn,
+// Two sums over the threads of a row (the first where `both`), to all of them.  More than a warp: through one of two buffers in turn,
 // so that one barrier is enough.
 template <int TPR>
 struct RowSum
 {
   float2 (*buffer)[TPR / 32];
   int turn = 0;
-  __device__ __forceinline__ float2 operator()(float a, float b)
+  __device__ __forceinline__ float2 operator()(float a, float b, bool both)
   {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
-    {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
       b += __shfl_xor_sync(0xffffffffu, b, o);
+    if (both)
+    {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        a += __shfl_xor_sync(0xffffffffu, a, o);
     }
     if (TPR == 32)
       return make_float2(a, b);
@@ -154,7 +167,7 @@ __device__ __forceinline__ float2 standardise(float (&v)[N], const NormParams& P
 #pragma unroll
     for (int i = 0; i < N; ++i)
       s += v[i];
-    mean = sum(s, 0.0f).x * P.inv_width;
+    mean = sum(0.0f, s, false).y * P.inv_width;
 #pragma unroll
     for (int i = 0; i < N; ++i)
       v[i] = column<WIDE, TPR>(t, i) < (int)P.width ? v[i] - mean : 0.0f;
@@ -163,7 +176,7 @@ __device__ __forceinline__ float2 standardise(float (&v)[N], const NormParams& P
 #pragma unroll
   for (int i = 0; i < N; ++i)
     s = fmaf(v[i], v[i], s);
-  const float rstd = 1.0f / sqrtf(sum(s, 0.0f).x * P.inv_width + P.eps);
+  const float rstd = 1.0f / sqrtf(sum(0.0f, s, false).y * P.inv_width + P.eps);
   return make_float2(mean, rstd);
 }
 
@@ -247,176 +260,413 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads) norm_forward_kernel(cons
     P.stats[row] = make_float4(first.x, first.y, second.x, second.y);
 }
 
-// 0 outside the row, where v - mean would not be
-template <bool WIDE, int TPR, int N>
-__device__ __forceinline__ void normalise(float (&v)[N], float mean, float rstd, int width, int t)
+// Backward works on pairs of neighbours (elements 2i and 2i + 1 of a thread).
+template <typename T, bool WIDE, int TPR, int M>
+__device__ __forceinline__ void load_pairs(const void* base, int64_t offset, int width, int t, float2x (&v)[M])
 {
+  const T* p = static_cast<const T*>(base) + offset;
+  if constexpr (WIDE)
+  {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    v[i] = column<WIDE, TPR>(t, i) < width ? (v[i] - mean) * rstd : 0.0f;
+    for (int i = 0; i < M; i += 4)
+    {
+      const int c = column<WIDE, TPR>(t, 2 * i);
+      if constexpr (sizeof(T) == 2)
+      {
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (c < width)
+          r = *reinterpret_cast<const uint4*>(p + c);
+        v[i] = pair_of_bf16(r.x), v[i + 1] = pair_of_bf16(r.y), v[i + 2] = pair_of_bf16(r.z), v[i + 3] = pair_of_bf16(r.w);
+      }
+      else
+      {
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+        if (c < width)
+          a = reinterpret_cast<const float4*>(p + c)[0], b = reinterpret_cast<const float4*>(p + c)[1];
+        v[i] = pair(a.x, a.y), v[i + 1] = pair(a.z, a.w), v[i + 2] = pair(b.x, b.y), v[i + 3] = pair(b.z, b.w);
+      }
+    }
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+    {
+      const int c = column<WIDE, TPR>(t, 2 * i), d = column<WIDE, TPR>(t, 2 * i + 1);
+      v[i] = pair(c < width ? to_float(p[c]) : 0.0f, d < width ? to_float(p[d]) : 0.0f);
+    }
+  }
 }
 
-template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
-__global__ void __launch_bounds__(Shape<TPR>::kThreads, TPR <= 256 ? 512 / Shape<TPR>::kThreads : 1)
+template <typename T, bool WIDE, int TPR, int M>
+__device__ __forceinline__ void store_pairs(void* base, int64_t offset, int width, int t, const float2x (&v)[M])
+{
+  T* p = static_cast<T*>(base) + offset;
+  if constexpr (WIDE)
+  {
+#pragma unroll
+    for (int i = 0; i < M; i += 4)
+    {
+      const int c = column<WIDE, TPR>(t, 2 * i);
+      if (c < width)
+      {
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint4*>(p + c) = make_uint4(bf16_of_pair(v[i]), bf16_of_pair(v[i + 1]), bf16_of_pair(v[i + 2]),
+                                                        bf16_of_pair(v[i + 3]));
+        else
+        {
+          const float2 a = halves(v[i]), b = halves(v[i + 1]), e = halves(v[i + 2]), f = halves(v[i + 3]);
+          reinterpret_cast<float4*>(p + c)[0] = make_float4(a.x, a.y, b.x, b.y);
+          reinterpret_cast<float4*>(p + c)[1] = make_float4(e.x, e.y, f.x, f.y);
+        }
+      }
+    }
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+    {
+      const int c = column<WIDE, TPR>(t, 2 * i), d = column<WIDE, TPR>(t, 2 * i + 1);
+      const float2 f = halves(v[i]);
+      if (c < width)
+        p[c] = from_float<T>(f.x);
+      if (d < width)
+        p[d] = from_float<T>(f.y);
+    }
+  }
+}
+
+template <int M>
+__device__ __forceinline__ void normalise(float2x (&v)[M], float mean, float rstd, bool layer)
+{
+  if (layer)
+  {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      v[i] = add2(v[i], pair(-mean));
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    v[i] = mul2(v[i], pair(rstd));
+}
+
+// The means over the row that the gradient of a norm takes off: of q (layer norms) and of q n.
+template <int TPR, int M>
+__device__ __forceinline__ float2 means(const float2x (&q)[M], const float2x (&n)[M], const NormParams& P, RowSum<TPR>& sum)
+{
+  float2x s1 = 0, s2 = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    s2 = fma2(q[i], n[i], s2);
+  if (P.layer)
+  {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      s1 = add2(s1, q[i]);
+  }
+  const float2 a = halves(s1), b = halves(s2);
+  const float2 all = sum(a.x + a.y, b.x + b.y, P.layer != 0);
+  return make_float2(all.x * P.inv_width, all.y * P.inv_width);
+}
+
+// q - <q> - n <q n>
+template <int M>
+__device__ __forceinline__ void take_off(float2x (&q)[M], const float2x (&n)[M], float2 mean, bool layer)
+{
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    q[i] = fma2(n[i], pair(-mean.y), q[i]);
+  if (layer)
+  {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      q[i] = add2(q[i], pair(-mean.x));
+  }
+}
+
+// The rows of a unit in their order: chunk after chunk, `units` apart.
+struct Cursor
+{
+  int chunk, row, end, group;
+  __device__ __forceinline__ void open(const NormParams& P)
+  {
+    if (chunk >= P.chunks)
+      return;
+    group = chunk / P.chunks_per_group;
+    row = group * P.rows_per_group + (chunk - group * P.chunks_per_group) * P.rows_per_chunk;
+    const int last = (group + 1) * P.rows_per_group;
+    end = last - row > P.rows_per_chunk ? row + P.rows_per_chunk : last;
+  }
+  __device__ __forceinline__ bool valid(const NormParams& P) const { return chunk < P.chunks; }
+  __device__ __forceinline__ void next(const NormParams& P)
+  {
+    if (++row == end)
+    {
+      chunk += P.units;
+      open(P);
+    }
+  }
+};
+
+constexpr int kFetched = 4; // new stream, d_normed, d_new_stream, branch
+
+// STAGES > 0: rows are fetched that many ahead.  The slot of a row is filled again after the first sum over the
+// next row, which every thread reaches after its last read of the slot.
+template <typename T, bool WIDE, int TPR, int VPT, bool BIAS, int STAGES>
+__global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThreads)
     norm_backward_kernel(const NormParams P)
 {
-  constexpr int N = VPT * 8;
+  constexpr int M = VPT * 4, kUnits = Shape<TPR>::kUnits;
+  constexpr bool kAhead = STAGES > 0;
   __shared__ float2 buffer[2][TPR / 32];
+  __shared__ uint64_t filled[kUnits][kAhead ? STAGES : 1];
+  __shared__ __align__(16) int give_up[4];
+  __shared__ Cursor ahead[kUnits]; // the next row to fetch: kept by thread 0 of a unit, out of the others' registers
+  extern __shared__ __align__(128) uint8_t slots[];
   RowSum<TPR> sum{buffer};
-  const int t = threadIdx.x & (TPR - 1), width = (int)P.width;
-  const int64_t unit = (int64_t)blockIdx.x * Shape<TPR>::kUnits + threadIdx.x / TPR;
+  const int t = threadIdx.x & (TPR - 1), width = (int)P.width, local = threadIdx.x / TPR;
+  const int unit = blockIdx.x * kUnits + local;
+  const uint32_t row_bytes = (uint32_t)(width * sizeof(T));
+  const uint32_t slot_at = local * STAGES * kFetched * row_bytes;
+  uint64_t* full = filled[local];
+  if (kAhead)
+  {
+    if (threadIdx.x == 0)
+    {
+      for (int u = 0; u < kUnits; ++u)
+        for (int s = 0; s < STAGES; ++s)
+          dpc::ptx::mbar_init(&filled[u][s], 1);
+      give_up[0] = 0;
+      *reinterpret_cast<long long*>(give_up + 2) = dpc::ptx::kWaitCyclesDefault;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+  }
   if (unit >= P.units)
     return;
-  float dwn[N] = {}, dwp[N] = {}, dbn[BIAS ? N : 1] = {}, dbp[BIAS ? N : 1] = {};
-  for (int64_t chunk = unit; chunk < P.chunks; chunk += P.units)
+  auto fetch = [&](int64_t row, int s) { // by one thread of the unit
+    dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)));
+    auto copy = [&](int k, const void* from, int64_t ld) {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       dpc::ptx::smem_u32(slots) + slot_at + (s * kFetched + k) * row_bytes),
+                   "l"(static_cast<const T*>(from) + row * ld), "r"(row_bytes), "r"(dpc::ptx::smem_u32(&full[s]))
+                   : "memory");
+    };
+    copy(0, P.r, P.r_ld);
+    copy(1, P.dh, P.dh_ld);
+    if (P.dr)
+      copy(2, P.dr, P.dr_ld);
+    if (P.has_branch)
+      copy(3, P.y, P.y_ld);
+  };
+  Cursor now{unit, 0, 0, 0};
+  now.open(P);
+  if (kAhead && t == 0)
   {
-    const int64_t group = chunk / P.chunks_per_group;
-    const int64_t begin = group * P.rows_per_group + (chunk - group * P.chunks_per_group) * P.rows_per_chunk;
-    const int64_t last = (group + 1) * P.rows_per_group;
-    const int64_t end = begin + P.rows_per_chunk < last ? begin + P.rows_per_chunk : last;
-    float dg[N] = {};
-    for (int64_t row = begin; row < end; ++row)
+    Cursor c = now;
+    for (int s = 0; s < STAGES && c.valid(P); ++s, c.next(P))
+      fetch(c.row, s);
+    ahead[local] = c;
+  }
+  float2x dwn[M] = {}, dwp[M] = {}, dg[M] = {}, dbn[BIAS ? M : 1] = {}, dbp[BIAS ? M : 1] = {};
+  const bool layer = P.layer != 0;
+  bool used = false; // a row before this one has left its slot
+  for (int slot = 0, parity = 0; now.valid(P);)
+  {
+    const int64_t row = now.row;
+    float4 st = __ldg(P.stats + row);
+    bool there = true;
+    if constexpr (kAhead)
+      there = dpc::ptx::mbar_wait(&full[slot], parity, give_up);
+    if (!there) // a copy that is never seen to arrive: NaN
+      st = make_float4(NAN, NAN, NAN, NAN);
+    auto get = [&](int k, const void* base, int64_t ld, float2x(&v)[M]) {
+      if constexpr (kAhead)
+        load_pairs<T, WIDE, TPR>(slots + slot_at + ((slot * kFetched + k) * row_bytes), 0, width, t, v);
+      else
+        load_pairs<T, WIDE, TPR>(base, row * ld, width, t, v);
+    };
+    float2x n[M], q[M], w[M];
+    get(0, P.r, P.r_ld, n);
+    get(1, P.dh, P.dh_ld, q);
+    normalise(n, st.z, st.w, layer);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
     {
-      const float4 st = P.stats[row];
-      float n[N], q[N], w[N];
-      load_row<T, WIDE, TPR>(P.r, row * P.r_ld, width, t, n, 0.0f);
-      load_row<T, WIDE, TPR>(P.dh, row * P.dh_ld, width, t, q, 0.0f);
-      normalise<WIDE, TPR>(n, st.z, st.w, width, t);
+      dwn[i] = fma2(q[i], n[i], dwn[i]);
+      if (BIAS)
+        dbn[i] = add2(dbn[i], there ? q[i] : pair(NAN));
+    }
+    if (P.wn)
+    {
+      load_pairs<T, WIDE, TPR>(P.wn, 0, width, t, w);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < M; ++i)
+        q[i] = mul2(q[i], w[i]);
+    }
+    float2 mean = means(q, n, P, sum);
+    if (kAhead && t == 0)
+    {
+      Cursor c = ahead[local];
+      if (used && c.valid(P))
       {
-        dwn[i] = fmaf(q[i], n[i], dwn[i]);
-        if (BIAS)
-          dbn[i] += q[i];
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fetch(c.row, slot == 0 ? STAGES - 1 : slot - 1);
+        c.next(P);
+        ahead[local] = c;
       }
-      if (P.wn)
-      {
-        load_row<T, WIDE, TPR>(P.wn, 0, width, t, w, 0.0f);
+      used = true;
+    }
+    take_off(q, n, mean, layer);
+    // times 1/deviation; nothing outside the row: the second norm sums over q
+    auto scale = [&](int i) {
+      const float lo = column<WIDE, TPR>(t, 2 * i) < width ? st.w : 0.0f;
+      return pair(lo, WIDE ? lo : column<WIDE, TPR>(t, 2 * i + 1) < width ? st.w : 0.0f);
+    };
+    if (P.dr)
+    {
+      get(2, P.dr, P.dr_ld, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          q[i] *= w[i];
-      }
-      float s1 = 0.0f, s2 = 0.0f;
+      for (int i = 0; i < M; ++i)
+        q[i] = fma2(q[i], scale(i), w[i]);
+    }
+    else
+    {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        s1 += q[i], s2 = fmaf(q[i], n[i], s2);
-      float2 mean = sum(s1, s2);
-      mean.x = P.layer ? mean.x * P.inv_width : 0.0f, mean.y *= P.inv_width;
-      // (nothing outside the row: the second norm sums over q)
+      for (int i = 0; i < M; ++i)
+        q[i] = mul2(q[i], scale(i));
+    }
+    if (P.dx)
+    {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        q[i] = column<WIDE, TPR>(t, i) < width ? st.w * (q[i] - mean.x - n[i] * mean.y) : 0.0f;
-      if (P.dr)
-      {
-        load_row<T, WIDE, TPR>(P.dr, row * P.dr_ld, width, t, w, 0.0f);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          q[i] += w[i];
-      }
-      if (P.dx)
-      {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          w[i] = P.a * q[i];
-        store_row<T, WIDE, TPR>(P.dx, row * P.dx_ld, width, t, w);
-      }
-      if (!P.has_branch)
-        continue;
+      for (int i = 0; i < M; ++i)
+        w[i] = mul2(q[i], pair(P.a));
+      store_pairs<T, WIDE, TPR>(P.dx, (int64_t)row * P.dx_ld, width, t, w);
+    }
+    if (P.has_branch)
+    {
       // q: gradient of b g u from here on.  n: the branch, standardised where it has a norm
-      load_row<T, WIDE, TPR>(P.y, row * P.y_ld, width, t, n, 0.0f);
+      get(3, P.y, P.y_ld, n);
       if (P.post)
-        normalise<WIDE, TPR>(n, st.x, st.y, width, t);
+        normalise(n, st.x, st.y, layer);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        q[i] *= P.b;
+      for (int i = 0; i < M; ++i)
+        q[i] = mul2(q[i], pair(P.b));
       if (P.dg)
       {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          w[i] = n[i];
-        if (P.post)
-          affine<T, WIDE, TPR>(w, P.wp, P.bp, width, t);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          dg[i] = fmaf(q[i], w[i], dg[i]);
-      }
-      if (P.gate)
-      {
-        load_row<T, WIDE, TPR>(P.gate, group * P.gate_ld, width, t, w, 0.0f);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          q[i] *= w[i];
-      }
-      if (P.post)
-      {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
+        // dg += q (n wp + bp)
+        if (P.bp)
         {
-          dwp[i] = fmaf(q[i], n[i], dwp[i]);
-          if (BIAS)
-            dbp[i] += q[i];
+          load_pairs<T, WIDE, TPR>(P.bp, 0, width, t, w);
+#pragma unroll
+          for (int i = 0; i < M; ++i)
+            dg[i] = fma2(q[i], w[i], dg[i]);
         }
         if (P.wp)
         {
-          load_row<T, WIDE, TPR>(P.wp, 0, width, t, w, 0.0f);
+          load_pairs<T, WIDE, TPR>(P.wp, 0, width, t, w);
 #pragma unroll
-          for (int i = 0; i < N; ++i)
-            q[i] *= w[i];
+          for (int i = 0; i < M; ++i)
+            dg[i] = fma2(q[i], mul2(w[i], n[i]), dg[i]);
         }
-        s1 = 0.0f, s2 = 0.0f;
+        else
+        {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          s1 += q[i], s2 = fmaf(q[i], n[i], s2);
-        mean = sum(s1, s2);
-        mean.x = P.layer ? mean.x * P.inv_width : 0.0f, mean.y *= P.inv_width;
+          for (int i = 0; i < M; ++i)
+            dg[i] = fma2(q[i], n[i], dg[i]);
+        }
+      }
+      if (P.gate)
+      {
+        load_pairs<T, WIDE, TPR>(P.gate, (int64_t)now.group * P.gate_ld, width, t, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          q[i] = st.y * (q[i] - mean.x - n[i] * mean.y);
+        for (int i = 0; i < M; ++i)
+          q[i] = mul2(q[i], w[i]);
+      }
+      if (P.post)
+      {
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+        {
+          dwp[i] = fma2(q[i], n[i], dwp[i]);
+          if (BIAS)
+            dbp[i] = add2(dbp[i], q[i]);
+        }
+        if (P.wp)
+        {
+          load_pairs<T, WIDE, TPR>(P.wp, 0, width, t, w);
+#pragma unroll
+          for (int i = 0; i < M; ++i)
+            q[i] = mul2(q[i], w[i]);
+        }
+        mean = means(q, n, P, sum);
+        take_off(q, n, mean, layer);
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+          q[i] = mul2(q[i], pair(st.y));
       }
       if (P.dy)
-        store_row<T, WIDE, TPR>(P.dy, row * P.dy_ld, width, t, q);
+        store_pairs<T, WIDE, TPR>(P.dy, (int64_t)row * P.dy_ld, width, t, q);
     }
-    if (P.dg)
+    if (++slot == STAGES || !kAhead)
+      slot = 0, parity ^= 1;
+    const int chunk = now.chunk, group = now.group;
+    now.next(P);
+    if (now.chunk != chunk && P.dg)
     {
       if (P.chunks_per_group == 1)
-        store_row<T, WIDE, TPR>(P.dg, group * P.dg_ld, width, t, dg);
+        store_pairs<T, WIDE, TPR>(P.dg, (int64_t)group * P.dg_ld, width, t, dg);
       else
-        store_row<float, WIDE, TPR>(P.gate_sums, chunk * width, width, t, dg);
+        store_pairs<float, WIDE, TPR>(P.gate_sums, (int64_t)chunk * P.sums_ld, width, t, dg);
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+        dg[i] = 0;
     }
   }
-  const int64_t plane = P.units * width, at = unit * width;
-  store_row<float, WIDE, TPR>(P.sums, at, width, t, dwn);
-  store_row<float, WIDE, TPR>(P.sums, at + plane, width, t, dwp);
-  if (BIAS)
+  const int64_t plane = P.units * P.sums_ld, at = unit * P.sums_ld;
+  store_pairs<float, WIDE, TPR>(P.sums, at, width, t, dwn);
+  store_pairs<float, WIDE, TPR>(P.sums, at + plane, width, t, dwp);
+  if constexpr (BIAS)
   {
-    store_row<float, WIDE, TPR, N>(P.sums, at + 2 * plane, width, t, reinterpret_cast<const float(&)[N]>(dbn));
-    store_row<float, WIDE, TPR, N>(P.sums, at + 3 * plane, width, t, reinterpret_cast<const float(&)[N]>(dbp));
+    store_pairs<float, WIDE, TPR>(P.sums, at + 2 * plane, width, t, dbn);
+    store_pairs<float, WIDE, TPR>(P.sums, at + 3 * plane, width, t, dbp);
+  }
+  if (kAhead && give_up[0])
+  {
+    // Copies that were not seen to arrive land before the block's shared memory goes away.
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL * STAGES)
+    {
+    }
   }
 }
 
-// Adds the units' sums: vector blockIdx.y of 32 columns a block; the first four are weights and biases, the
+// Adds the units' sums: vector blockIdx.y, 128 columns a block; the first four are weights and biases, the
 // others the gates.
 struct JoinParams
 {
   const float *sums, *gate_sums;
-  int64_t units, width, chunks_per_group, dg_ld;
+  int64_t units, width, ld, chunks_per_group, dg_ld;
   void* out[4];
   void* dg;
 };
 
+constexpr int kJoinWarps = 32;
+
 template <typename T>
-__global__ void __launch_bounds__(256) norm_join_kernel(const JoinParams P)
+__global__ void __launch_bounds__(32 * kJoinWarps) norm_join_kernel(const JoinParams P)
 {
-  __shared__ float parts[8][33];
+  __shared__ float4 parts[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t col = (int64_t)blockIdx.x * 128 + 4 * lane;
   const float* src;
   T* out;
   int64_t count;
   if (blockIdx.y < 4)
   {
     out = static_cast<T*>(P.out[blockIdx.y]);
-    src = P.sums + blockIdx.y * P.units * P.width, count = P.units;
+    src = P.sums + blockIdx.y * P.units * P.ld, count = P.units;
     if (!out)
       return;
   }
@@ -424,29 +674,43 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const JoinParams P)
   {
     const int64_t group = blockIdx.y - 4;
     out = static_cast<T*>(P.dg) + group * P.dg_ld;
-    src = P.gate_sums + group * P.chunks_per_group * P.width, count = P.chunks_per_group;
+    src = P.gate_sums + group * P.chunks_per_group * P.ld, count = P.chunks_per_group;
   }
-  float s = 0.0f;
-  if (col < P.width)
-    for (int64_t u = warp; u < count; u += 8)
-      s += src[u * P.width + col];
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (col < P.ld)
+  {
+#pragma unroll 8
+    for (int64_t u = warp; u < count; u += kJoinWarps)
+    {
+      const float4 v = *reinterpret_cast<const float4*>(src + u * P.ld + col);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+  }
   parts[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < P.width)
+  if (threadIdx.x < 128)
   {
-    s = 0.0f;
+    const float* all = reinterpret_cast<const float*>(parts);
+    float total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w)
-      s += parts[w][lane];
-    out[col] = from_float<T>(s);
+    for (int w = 0; w < kJoinWarps; ++w)
+      total += all[w * 128 + threadIdx.x];
+    const int64_t mine = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (mine < P.width)
+      out[mine] = from_float<T>(total);
   }
 }
 
 // ------------------------------------------------------------------------------ host
 int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-// Threads of a row: two vectors of 8 a thread, four in the widest rows.
-int threads_of(int64_t width) { return width <= 512 ? 32 : width <= 2048 ? 128 : width <= 4096 ? 256 : 512; }
+// Threads of a row.  Two vectors of 8 a thread, four in the widest rows; one, as far as 512 threads go, in backward
+// passes that keep sums of biases or load element by element (`lean`): two would not fit their registers.
+int threads_of(int64_t width, bool lean)
+{
+  const int64_t each = lean ? 8 : 16;
+  return width <= 32 * each ? 32 : width <= 128 * each ? 128 : width <= 256 * each ? 256 : 512;
+}
 
 struct Split
 {
@@ -455,25 +719,27 @@ struct Split
   size_t gate_at = 0, bytes = 0;
 };
 
-int split_rows(const dpc_residual_norm* c, Split& S)
+int split_rows(const dpc_residual_norm* c, bool lean, Split& S)
 {
   int device = 0, sms = 0;
   DPC_CUDA(cudaGetDevice(&device));
   DPC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   // Units that the GPU holds at once: 512 threads an SM, the registers of the kernel allow no more.
-  const int64_t most = (int64_t)sms * (512 / threads_of(c->width));
+  const int64_t most = (int64_t)sms * (512 / threads_of(c->width, lean));
   const int64_t groups = c->gate ? c->groups : 1, per = c->rows / groups;
-  S.chunks_per_group = std::max<int64_t>(1, std::min(per, most / groups));
+  // (four rows to a unit at least: its sums are written and read again)
+  S.chunks_per_group = std::max<int64_t>(1, std::min(ceil_div(per, 4), most / groups));
   S.rows_per_chunk = std::max<int64_t>(1, ceil_div(per, S.chunks_per_group));
   S.chunks_per_group = std::max<int64_t>(1, ceil_div(per, S.rows_per_chunk));
   S.chunks = S.chunks_per_group * groups;
   S.units = std::min(S.chunks, most);
   S.gates = c->gate && S.chunks_per_group > 1;
-  size_t at = (size_t)S.units * c->width * 4 * sizeof(float);
+  const int64_t ld = ceil_div(c->width, 8) * 8;
+  size_t at = (size_t)S.units * ld * 4 * sizeof(float);
   at = (at + 255) / 256 * 256;
   S.gate_at = at;
   if (S.gates)
-    at += (size_t)S.chunks * c->width * sizeof(float);
+    at += (size_t)S.chunks * ld * sizeof(float);
   S.bytes = std::max<size_t>(at, 256);
   return DPC_OK;
 }
@@ -491,8 +757,8 @@ int check(const dpc_residual_norm* c, const std::string& who)
   if (c->width > kMaxWidth)
     return dpc::fail(DPC_ERR_TOO_LARGE, who + ": width is " + std::to_string(c->width) + ", " +
                                             std::to_string(kMaxWidth) + " at most");
-  if (c->rows > (int64_t)1 << 31)
-    return dpc::fail(DPC_ERR_TOO_LARGE, who + ": rows may be 2^31 at most");
+  if (c->rows >= (int64_t)1 << 31)
+    return dpc::fail(DPC_ERR_TOO_LARGE, who + ": rows have to be below 2^31");
   if (c->gate && (c->groups < 1 || c->rows % c->groups != 0 || c->gate_stride < c->width))
     return dpc::fail(DPC_ERR_INVALID, who + ": the gate's groups have to divide the rows, and its rows not to overlap");
   if (!c->branch && (c->gate || c->post_norm || c->post_weight || c->post_bias || c->stream_scale != 1.0f))
@@ -526,7 +792,7 @@ NormParams params(const dpc_residual_norm* c)
 {
   NormParams P = {};
   P.rows = c->rows, P.width = c->width;
-  P.rows_per_group = std::max<int64_t>(1, c->gate ? c->rows / c->groups : c->rows);
+  P.rows_per_group = (int)std::max<int64_t>(1, c->gate ? c->rows / c->groups : c->rows);
   P.layer = c->norm == DPC_NORM_LAYER, P.post = c->post_norm != 0, P.has_branch = c->branch != nullptr;
   P.a = c->stream_scale, P.b = c->branch_scale, P.eps = c->eps, P.inv_width = 1.0f / (float)c->width;
   P.x = c->stream, P.y = c->branch, P.gate = c->gate;
@@ -546,33 +812,75 @@ int launch_forward(cudaStream_t stream, const NormParams& P)
   return launched("norm_forward_kernel");
 }
 
-template <typename T, bool WIDE, int TPR, int VPT>
-int launch_backward(cudaStream_t stream, const NormParams& P, bool bias)
+template <typename T, bool WIDE, int TPR, int VPT, bool BIAS, int STAGES>
+int launch_backward(cudaStream_t stream, const NormParams& P)
 {
+  auto kernel = norm_backward_kernel<T, WIDE, TPR, VPT, BIAS, STAGES>;
   const unsigned blocks = (unsigned)ceil_div(P.units, Shape<TPR>::kUnits);
-  if (bias)
-    norm_backward_kernel<T, WIDE, TPR, VPT, true><<<blocks, Shape<TPR>::kThreads, 0, stream>>>(P);
-  else
-    norm_backward_kernel<T, WIDE, TPR, VPT, false><<<blocks, Shape<TPR>::kThreads, 0, stream>>>(P);
+  const size_t bytes = (size_t)Shape<TPR>::kUnits * STAGES * kFetched * P.width * sizeof(T);
+  if (STAGES > 0)
+    DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  kernel<<<blocks, Shape<TPR>::kThreads, bytes, stream>>>(P);
   return launched("norm_backward_kernel");
+}
+
+template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
+int launch_backward(cudaStream_t stream, const NormParams& P)
+{
+  if constexpr (WIDE)
+  {
+    // Three rows ahead where the blocks of an SM have the shared memory for them, two, or none.
+    const size_t row = (size_t)512 / TPR * kFetched * P.width * sizeof(T), have = 200 << 10;
+    if (row * 3 <= have)
+      return launch_backward<T, true, TPR, VPT, BIAS, 3>(stream, P);
+    if (row * 2 <= have)
+      return launch_backward<T, true, TPR, VPT, BIAS, 2>(stream, P);
+  }
+  return launch_backward<T, WIDE, TPR, VPT, BIAS, 0>(stream, P);
+}
+
+template <typename T, bool WIDE>
+int dispatch_forward(cudaStream_t stream, const NormParams& P)
+{
+  switch (threads_of(P.width, false))
+  {
+  case 32:
+    return launch_forward<T, WIDE, 32, 2>(stream, P);
+  case 128:
+    return launch_forward<T, WIDE, 128, 2>(stream, P);
+  case 256:
+    return launch_forward<T, WIDE, 256, 2>(stream, P);
+  default:
+    return P.width <= 8192 ? launch_forward<T, WIDE, 512, 2>(stream, P) : launch_forward<T, WIDE, 512, 4>(stream, P);
+  }
+}
+
+template <typename T, bool WIDE, bool BIAS>
+int dispatch_backward(cudaStream_t stream, const NormParams& P)
+{
+  constexpr bool kLean = BIAS || !WIDE;
+  constexpr int VPT = kLean ? 1 : 2;
+  switch (threads_of(P.width, kLean))
+  {
+  case 32:
+    return launch_backward<T, WIDE, 32, VPT, BIAS>(stream, P);
+  case 128:
+    return launch_backward<T, WIDE, 128, VPT, BIAS>(stream, P);
+  case 256:
+    return launch_backward<T, WIDE, 256, VPT, BIAS>(stream, P);
+  default:
+    return P.width <= 512 * VPT * 8 ? launch_backward<T, WIDE, 512, VPT, BIAS>(stream, P)
+           : P.width <= 8192        ? launch_backward<T, WIDE, 512, 2, BIAS>(stream, P)
+                                    : launch_backward<T, WIDE, 512, 4, BIAS>(stream, P);
+  }
 }
 
 template <typename T, bool WIDE>
 int dispatch(cudaStream_t stream, const NormParams& P, bool back, bool bias)
 {
-  switch (threads_of(P.width))
-  {
-  case 32:
-    return back ? launch_backward<T, WIDE, 32, 2>(stream, P, bias) : launch_forward<T, WIDE, 32, 2>(stream, P);
-  case 128:
-    return back ? launch_backward<T, WIDE, 128, 2>(stream, P, bias) : launch_forward<T, WIDE, 128, 2>(stream, P);
-  case 256:
-    return back ? launch_backward<T, WIDE, 256, 2>(stream, P, bias) : launch_forward<T, WIDE, 256, 2>(stream, P);
-  default:
-    if (P.width <= 8192)
-      return back ? launch_backward<T, WIDE, 512, 2>(stream, P, bias) : launch_forward<T, WIDE, 512, 2>(stream, P);
-    return back ? launch_backward<T, WIDE, 512, 4>(stream, P, bias) : launch_forward<T, WIDE, 512, 4>(stream, P);
-  }
+  if (!back)
+    return dispatch_forward<T, WIDE>(stream, P);
+  return bias ? dispatch_backward<T, WIDE, true>(stream, P) : dispatch_backward<T, WIDE, false>(stream, P);
 }
 
 int dispatch(cudaStream_t stream, int type, bool is_wide, const NormParams& P, bool back, bool bias)
@@ -582,6 +890,16 @@ int dispatch(cudaStream_t stream, int type, bool is_wide, const NormParams& P, b
   return is_wide ? dispatch<__nv_bfloat16, true>(stream, P, back, bias)
                  : dispatch<__nv_bfloat16, false>(stream, P, back, bias);
 }
+
+bool wide_backward(const dpc_residual_norm* c)
+{
+  return wide(c, {{c->branch, c->branch_stride}, {c->gate, c->gate_stride}, {c->new_stream, c->new_stream_stride},
+                  {c->d_normed, c->d_normed_stride}, {c->d_new_stream, c->d_new_stream_stride},
+                  {c->d_stream, c->d_stream_stride}, {c->d_branch, c->d_branch_stride}, {c->d_gate, c->d_gate_stride},
+                  {c->post_weight, 0}, {c->post_bias, 0}, {c->pre_weight, 0}});
+}
+
+bool with_bias(const dpc_residual_norm* c) { return c->d_post_bias || c->d_pre_bias; }
 
 int forward(cudaStream_t stream, const dpc_residual_norm* c)
 {
@@ -632,8 +950,9 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
                                       {c->d_normed, c->d_normed_stride}, {c->d_new_stream, c->d_new_stream_stride},
                                       {c->d_stream, c->d_stream_stride}, {c->d_branch, c->d_branch_stride}}))
     return rc;
+  const bool w = wide_backward(c);
   Split S;
-  if (int rc = split_rows(c, S))
+  if (int rc = split_rows(c, with_bias(c) || !w, S))
     return rc;
   if (!c->workspace || reinterpret_cast<uintptr_t>(c->workspace) % 256 || c->workspace_bytes < S.bytes)
     return dpc::fail(DPC_ERR_INVALID, who + ": " + std::to_string(S.bytes) +
@@ -642,26 +961,23 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
   P.dh = c->d_normed, P.dr = c->d_new_stream, P.dx = c->d_stream, P.dy = c->d_branch, P.dg = c->d_gate;
   P.dh_ld = c->d_normed_stride, P.dr_ld = c->d_new_stream_stride, P.dx_ld = c->d_stream_stride;
   P.dy_ld = c->d_branch_stride, P.dg_ld = c->d_gate_stride;
-  P.units = S.units, P.chunks = S.chunks, P.chunks_per_group = S.chunks_per_group, P.rows_per_chunk = S.rows_per_chunk;
+  P.units = (int)S.units, P.chunks = (int)S.chunks;
+  P.chunks_per_group = (int)S.chunks_per_group, P.rows_per_chunk = (int)S.rows_per_chunk;
+  P.sums_ld = ceil_div(c->width, 8) * 8;
   P.sums = static_cast<float*>(c->workspace);
   P.gate_sums = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + S.gate_at);
-  const bool w = wide(c, {{c->branch, c->branch_stride}, {c->gate, c->gate_stride},
-                          {c->new_stream, c->new_stream_stride}, {c->d_normed, c->d_normed_stride},
-                          {c->d_new_stream, c->d_new_stream_stride}, {c->d_stream, c->d_stream_stride},
-                          {c->d_branch, c->d_branch_stride}, {c->d_gate, c->d_gate_stride}, {c->post_weight, 0},
-                          {c->post_bias, 0}, {c->pre_weight, 0}});
-  if (int rc = dispatch(stream, c->type, w, P, true, c->d_post_bias || c->d_pre_bias))
+  if (int rc = dispatch(stream, c->type, w, P, true, with_bias(c)))
     return rc;
   JoinParams J = {};
-  J.sums = P.sums, J.gate_sums = P.gate_sums, J.units = S.units, J.width = c->width;
+  J.sums = P.sums, J.gate_sums = P.gate_sums, J.units = S.units, J.width = c->width, J.ld = P.sums_ld;
   J.chunks_per_group = S.chunks_per_group, J.dg = c->d_gate, J.dg_ld = c->d_gate_stride;
   J.out[0] = c->d_pre_weight, J.out[1] = c->d_post_weight, J.out[2] = c->d_pre_bias, J.out[3] = c->d_post_bias;
   const int64_t vectors = 4 + (S.gates && c->d_gate ? c->groups : 0);
-  const dim3 grid((unsigned)ceil_div(c->width, 32), (unsigned)vectors); // (groups: fewer than units there)
+  const dim3 grid((unsigned)ceil_div(c->width, 128), (unsigned)vectors); // (groups: fewer than units there)
   if (c->type == DPC_TYPE_F32)
-    norm_join_kernel<float><<<grid, 256, 0, stream>>>(J);
+    norm_join_kernel<float><<<grid, 32 * kJoinWarps, 0, stream>>>(J);
   else
-    norm_join_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(J);
+    norm_join_kernel<__nv_bfloat16><<<grid, 32 * kJoinWarps, 0, stream>>>(J);
   return launched("norm_join_kernel");
 }
 } // namespace
@@ -679,7 +995,7 @@ int dpc_residual_norm_workspace(const dpc_residual_norm* c, size_t* bytes)
     if (int rc = check(c, "dpc_residual_norm_workspace"))
       return rc;
     Split S;
-    if (int rc = split_rows(c, S))
+    if (int rc = split_rows(c, with_bias(c) || !wide_backward(c), S))
       return rc;
     *bytes = S.bytes;
     return (int)DPC_OK;

@@ -70,6 +70,51 @@ __device__ __forceinline__ void store8w(float* p, const float* v)
 }
 __device__ __forceinline__ void store8w(__nv_bfloat16* p, const float* v) { *reinterpret_cast<uint4*>(p) = pack8(v); }
 
+// Two 32-bit floats in a register pair and the instructions that work on both at once: half the issue slots of
+// kernels whose arithmetic, not only their traffic, is near the limit.
+typedef unsigned long long float2x;
+__device__ __forceinline__ float2x pair(float a, float b)
+{
+  float2x r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2x pair(float a) { return pair(a, a); }
+__device__ __forceinline__ float2 halves(float2x v)
+{
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2x fma2(float2x a, float2x b, float2x c)
+{
+  float2x r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float2x mul2(float2x a, float2x b)
+{
+  float2x r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2x add2(float2x a, float2x b)
+{
+  float2x r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2x pair_of_bf16(uint32_t v)
+{
+  return pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t bf16_of_pair(float2x v)
+{
+  const float2 f = halves(v);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -677,7 +677,7 @@ typedef struct dpc_vocab_ce
   void* workspace;
   size_t workspace_bytes;
 } dpc_vocab_ce;
-/* Pointers of the description have to be those of the call: an operand off a 16-byte boundary is copied. */
+/* Pointers and strides of the description have to be those of the call: an operand off a 16-byte boundary is copied. */
 DPC_API int dpc_vocab_ce_workspace(const dpc_vocab_ce* call, int backward, size_t* bytes);
 DPC_API int dpc_vocab_ce_forward(void* stream, const dpc_vocab_ce* call);
 DPC_API int dpc_vocab_ce_backward(void* stream, const dpc_vocab_ce* call);
@@ -694,7 +694,7 @@ DPC_API int dpc_vocab_ce_backward(void* stream, const dpc_vocab_ce* call);
  * Backward reads new_stream, branch and stats: d_normed and d_new_stream (NULL: none) are the gradients
  * of the two outputs; d_branch, d_gate and the gradients of weights and biases are written where the
  * tensor is given (a gradient pointer may be NULL: not wanted).  width 16384 at most; rows may be 0 (vector gradients are
- * then zeros). */
+ * then zeros).  The workspace depends on pointers and strides too: ask with those of the call. */
 typedef enum dpc_norm
 {
   DPC_NORM_RMS = 0,

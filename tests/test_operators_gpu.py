@@ -452,7 +452,7 @@ def test_pack_activations(dp, act, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("rows,width", [(1, 1), (1, 7), (3, 8), (5, 127), (2, 128), (7, 129), (33, 1000), (300, 136), (1, 40000)])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 7), (3, 8), (5, 127), (2, 128), (7, 129), (33, 1000), (300, 136), (1, 40000), (9, 4096), (40, 272)])
 def test_pack_sizes(dp, rows, width, kind):
     g = gen(2)
     x = normal(g, rows, width, dtype=TYPES[kind])
