@@ -23,10 +23,12 @@
 // to bf16 themselves.
 //
 // 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low) in the six products
-// whose terms reach 2^-24, smallest first; s is held in as many planes.  The tensor cores truncate their 32-bit sums,
-// which over the 628 additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm); so a contraction is
-// cut into runs of 8 stages (32 additions) whose sums the epilogue warps add up in registers, rounded to
-// nearest.  They have registers for tiles 128 wide.
+// whose terms reach 2^-24; s is held in as many planes.  A stage holds the three planes of both operands, so
+// that six products are made of six loads (a pass over the operands for each product was bound by L2: 4096
+// bytes a step of 256 cycles and SM).  The tensor cores truncate their 32-bit sums, which over the 628
+// additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm); so hi x hi has an accumulator of its
+// own, and a contraction is cut into runs of 8 stages (32 additions) whose sums the epilogue warps add up
+// in registers, rounded to nearest.  They have registers for tiles 128 wide.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -57,12 +59,14 @@ constexpr int kRun = 8; // stages whose products the tensor cores add up, where 
 template <int COLS>
 struct Tile
 {
-  static constexpr int kABytes = kRows * kRowBytes, kBBytes = COLS / 2 * kRowBytes;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
   static constexpr bool kRuns = COLS < kTile;
-  static constexpr int kShare = COLS / 2; // columns of an epilogue warp
+  static constexpr int kPlanes = kRuns ? 3 : 1; // of each operand, in a stage
+  static constexpr int kABytes = kRows * kRowBytes, kBBytes = COLS / 2 * kRowBytes;
+  static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
+  static constexpr int kStages = kRuns ? 3 : 6;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+  static constexpr int kSets = kRuns ? 2 : 1; // accumulators of a tile: hi x hi, and the five smaller products
+  static constexpr int kShare = COLS / 2;     // columns of an epilogue warp
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -80,8 +84,7 @@ enum Epilogue
 struct GemmParams
 {
   int64_t tiles_m, tiles_n, group_m, items; // items = splits * tiles_m * tiles_n
-  int splits, kblocks, passes;
-  uint32_t plane_a, plane_b; // plane of a pass, 4 bits each
+  int splits, kblocks;
   int64_t m, n;              // rows and columns of the product
   // logits
   float factor;     // scale * log2(e)
@@ -135,8 +138,7 @@ __device__ __forceinline__ void locate(const GemmParams& P, int64_t item, int& s
 
 __device__ __forceinline__ void range_of(const GemmParams& P, int split, int& begin, int& end)
 {
-  const int64_t total = (int64_t)P.kblocks * P.passes;
-  begin = (int)(total * split / P.splits), end = (int)(total * (split + 1) / P.splits);
+  begin = (int)((int64_t)P.kblocks * split / P.splits), end = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
 }
 
 // 32 logits of a row in units of log 2, -inf outside the vocabulary.
@@ -175,7 +177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 {
   using C = Tile<COLS>;
   constexpr int kStages = C::kStages, kStageBytes = C::kStageBytes;
-  constexpr uint32_t kTmemColumns = 2 * COLS;
+  constexpr uint32_t kTmemColumns = 2 * C::kSets * COLS;
   constexpr uint32_t kInstr = (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
                               ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(COLS >> 3) << 17) |
                               ((uint32_t)(kTile >> 4) << 24);
@@ -242,7 +244,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         locate(P, item, split, tm, tn);
         range_of(P, split, it, it_end);
         const int m0 = (int)(tm * kTile) + (int)rank * kRows, n0 = (int)(tn * COLS) + (int)rank * (COLS / 2);
-        int pass = it / P.kblocks, kb = it - pass * P.kblocks;
         for (; it < it_end; ++it)
         {
           if (!mbar_wait_cluster(&empty[s], phase, abort_flag))
@@ -254,26 +255,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_expect_tx(&full[s], 2 * kStageBytes); // both CTAs' copies count on the leader's barrier
           const uint32_t bar = lead_full + (uint32_t)(s * 8);
           uint8_t* a = stages + s * kStageBytes;
-          uint8_t* b = a + C::kABytes;
-          const int pa = (P.plane_a >> (4 * pass)) & 15, pb = (P.plane_b >> (4 * pass)) & 15;
-          const int k = kb * kDepth;
-          if (A_MN)
+          uint8_t* b = a + C::kPlanes * C::kABytes;
+          const int k = it * kDepth;
+#pragma unroll
+          for (int pl = 0; pl < C::kPlanes; ++pl, a += C::kABytes, b += C::kBBytes)
           {
-            tma_load_3d_pair(a, &map_a, bar, m0, k, pa);
-            tma_load_3d_pair(a + 64 * kRowBytes, &map_a, bar, m0 + 64, k, pa);
+            if (A_MN)
+            {
+              tma_load_3d_pair(a, &map_a, bar, m0, k, pl);
+              tma_load_3d_pair(a + 64 * kRowBytes, &map_a, bar, m0 + 64, k, pl);
+            }
+            else
+              tma_load_3d_pair(a, &map_a, bar, k, m0, pl);
+            tma_load_3d_pair(b, &map_b, bar, B_MN ? n0 : k, B_MN ? k : n0, pl);
+            if (B_MN && COLS == 256)
+              tma_load_3d_pair(b + 64 * kRowBytes, &map_b, bar, n0 + 64, k, pl);
           }
-          else
-            tma_load_3d_pair(a, &map_a, bar, k, m0, pa);
-          if (B_MN)
-          {
-            tma_load_3d_pair(b, &map_b, bar, n0, k, pb);
-            if (COLS == 256)
-              tma_load_3d_pair(b + 64 * kRowBytes, &map_b, bar, n0 + 64, k, pb);
-          }
-          else
-            tma_load_3d_pair(b, &map_b, bar, k, n0, pb);
-          if (++kb == P.kblocks)
-            kb = 0, ++pass;
           if (++s == kStages)
             s = 0, phase ^= 1;
         }
@@ -296,7 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // K-major: rows of 128 bytes, 8 to a swizzle atom.  MN-major: blocks of 64 columns (8 KB apart) of
       // 64 k-rows, 8 k-rows to an atom, 16 k-rows to an instruction.
       const uint64_t da0 = make_desc(smem_u32(stages), A_MN ? 64 * kRowBytes : 16, 1024, 2);
-      const uint64_t db0 = make_desc(smem_u32(stages) + C::kABytes, B_MN ? 64 * kRowBytes : 16, 1024, 2);
+      const uint64_t db0 = make_desc(smem_u32(stages) + C::kPlanes * C::kABytes, B_MN ? 64 * kRowBytes : 16, 1024, 2);
       constexpr uint32_t adv_a = (A_MN ? 2048 : 32) >> 4, adv_b = (B_MN ? 2048 : 32) >> 4;
       int s = 0, turn = 0;
       uint32_t phase = 0;
@@ -316,7 +313,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           ++turn;
           tc_fence_after();
-          const uint32_t d = tmem_base + acc * COLS;
+          const uint32_t d = tmem_base + acc * (C::kSets * COLS);
           for (uint32_t more = 0; it < run_end; ++it)
           {
             if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[s], phase, abort_flag)))
@@ -329,7 +326,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < kDepth / 16; ++ks)
             {
-              tc_mma_bf16_pair(d, sa + (uint64_t)(ks * adv_a), sb + (uint64_t)(ks * adv_b), kInstr, more);
+              const uint64_t a = sa + (uint64_t)(ks * adv_a), b = sb + (uint64_t)(ks * adv_b);
+              if (C::kRuns)
+              {
+                constexpr uint64_t pa = C::kABytes >> 4, pb = C::kBBytes >> 4; // from plane to plane
+                tc_mma_bf16_pair(d + COLS, a + 2 * pa, b, kInstr, more);
+                tc_mma_bf16_pair(d + COLS, a, b + 2 * pb, kInstr, 1);
+                tc_mma_bf16_pair(d + COLS, a + pa, b + pb, kInstr, 1);
+                tc_mma_bf16_pair(d + COLS, a + pa, b, kInstr, 1);
+                tc_mma_bf16_pair(d + COLS, a, b + pb, kInstr, 1);
+              }
+              tc_mma_bf16_pair(d, a, b, kInstr, more);
               more = 1;
             }
             tc_commit_pair(smem_u32(&empty[s])); // the stage is free in both CTAs
@@ -391,7 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * COLS + half * C::kShare;
+          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + half * C::kShare;
 #pragma unroll
           for (int c = 0; c < C::kShare / 32; ++c)
           {
@@ -401,6 +408,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               sums[C::kRuns ? c : 0][i] = first ? v[i] : sums[C::kRuns ? c : 0][i] + v[i];
+            tc_ld32(taddr + COLS + 32 * c, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              sums[C::kRuns ? c : 0][i] += v[i];
           }
           tc_fence_before();
           __syncwarp();
@@ -413,7 +424,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         alive = __all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag));
       ++turn;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * COLS + half * C::kShare;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + half * C::kShare;
       const float out_factor = EPI == EPI_OUT ? *P.grad_top * P.scale : 1.0f;
       float top = -INFINITY, total = 0.0f;
 #pragma unroll(C::kRuns ? C::kShare / 32 : 1)
@@ -423,11 +434,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float v[32];
         __syncwarp();
         tc_ld32(taddr + 32 * c, v); // (a read of whatever is there, after a wait that gave up)
-        if (C::kRuns && several)
+        if (C::kRuns)
         {
+          float w[32];
+          tc_ld32(taddr + COLS + 32 * c, w);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            v[i] += sums[C::kRuns ? c : 0][i];
+            v[i] += several ? sums[C::kRuns ? c : 0][i] + w[i] : w[i];
         }
         if (!alive)
         {
@@ -567,6 +580,149 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
+// The parts of few rows without tensor cores: a tile of 256 rows would be all but empty, and the weights, read once,
+// are the whole cost (65 MB for 32000 words x 1024 in bf16: 10 us at the rate of a copy).  The rows lie in shared
+// memory in 32 bits; a warp multiplies them with kWords words at a time, 8 elements a lane and word, and keeps the
+// maximum and the sum of exponentials of what it has seen.  ROWS: rows, rounded up.  WIDE: 16-byte loads of the weights.
+// 32000 words x 1024, 1 / 2 / 4 / 8 rows: bf16 17 / 19 / 40 / 40 us where the tensor cores take 24, f32 24 / 26 / 31 / 43
+// us where they take 128 (52 of them for the planes): hence up to 2 and up to 8 rows.
+template <typename T>
+constexpr int kFewRows = sizeof(T) == 2 ? 2 : 8;
+constexpr int kWords = 4, kFewThreads = 256;
+constexpr size_t kFewBytes = 96 << 10; // shared memory for the rows: two blocks an SM
+
+template <typename T, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(kFewThreads, ROWS > 4 ? 1 : 2)
+    vocab_few_kernel(const T* __restrict__ hidden, int64_t hidden_ld, const T* __restrict__ weight, int64_t weight_ld,
+                     int rows, int width, int64_t vocab, const T* __restrict__ bias, float factor,
+                     const int64_t* __restrict__ targets, int64_t ignore_index, float2* __restrict__ partial,
+                     float* __restrict__ picked)
+{
+  extern __shared__ __align__(16) float held[]; // [rows][chunks of 256]
+  __shared__ float2 parts[kFewThreads / 32][ROWS];
+  const int chunks = (width + 255) / 256, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Element k of a row: chunk k / 256; WIDE: lane (k / 8) % 32, its first four and its last four apart, so that
+  // the lanes' 16-byte reads meet no bank twice; otherwise in order.
+  for (int r = 0; r < ROWS; ++r)
+    for (int k = threadIdx.x; k < chunks * 256; k += kFewThreads)
+    {
+      const int at = WIDE ? (k & ~255) + ((k >> 2) & 1) * 128 + ((k >> 3) & 31) * 4 + (k & 3) : k;
+      held[r * chunks * 256 + at] = r < rows && k < width ? to_float(hidden[r * hidden_ld + k]) : 0.0f;
+    }
+  float top[ROWS], total[ROWS];
+  int target[ROWS]; // (2^28 words at most)
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+  {
+    top[r] = -INFINITY, total[r] = 0.0f, target[r] = -1;
+    if (r < rows && counted(targets[r], vocab, ignore_index))
+      target[r] = (int)targets[r];
+  }
+  __syncthreads();
+  const int64_t step = (int64_t)gridDim.x * (kFewThreads / 32) * kWords;
+  for (int64_t word = ((int64_t)blockIdx.x * (kFewThreads / 32) + warp) * kWords; word < vocab; word += step)
+  {
+    float2x sum[kWords][ROWS] = {};
+#pragma unroll 2
+    for (int c = 0; c < chunks; ++c)
+    {
+      float2x w[kWords][4];
+#pragma unroll
+      for (int j = 0; j < kWords; ++j)
+      {
+        const T* p = weight + (word + j < vocab ? word + j : vocab - 1) * weight_ld; // (a word behind the last: not used)
+        float v[8];
+        if constexpr (WIDE)
+        {
+          const int k = c * 256 + lane * 8;
+          if (k < width)
+            load8w(p + k, v);
+          else
+          {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              v[i] = 0.0f;
+          }
+        }
+        else
+        {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+          {
+            const int k = c * 256 + i * 32 + lane;
+            v[i] = k < width ? to_float(p[k]) : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[j][i] = pair(v[2 * i], v[2 * i + 1]);
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+      {
+        const float* x = held + (r * chunks + c) * 256;
+        float2x h[4];
+        if constexpr (WIDE)
+        {
+          const float4 a = *reinterpret_cast<const float4*>(x + lane * 4), b = *reinterpret_cast<const float4*>(x + 128 + lane * 4);
+          h[0] = pair(a.x, a.y), h[1] = pair(a.z, a.w), h[2] = pair(b.x, b.y), h[3] = pair(b.z, b.w);
+        }
+        else
+        {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            h[i] = pair(x[i * 64 + lane], x[i * 64 + 32 + lane]);
+        }
+#pragma unroll
+        for (int j = 0; j < kWords; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sum[j][r] = fma2(w[j][i], h[i], sum[j][r]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kWords; ++j)
+    {
+      if (word + j >= vocab)
+        break;
+      const float b = bias ? to_float(bias[word + j]) * kLog2e : 0.0f;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+      {
+        const float2 both = halves(sum[j][r]);
+        float l = both.x + both.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          l += __shfl_xor_sync(0xffffffffu, l, o);
+        l = bias ? fmaf(l, factor, b) : l * factor;
+        if (word + j == target[r] && lane == 0)
+          picked[r] = l;
+        // (nothing but -inf so far: zero in its place leaves the sum at 0, or NaN where a logit is NaN)
+        const float most = fmaxf(top[r], l), base = most == -INFINITY ? 0.0f : most;
+        total[r] = fmaf(total[r], ex2(top[r] - base), ex2(l - base));
+        top[r] = most;
+      }
+    }
+  }
+  if (lane == 0)
+  {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      parts[warp][r] = make_float2(top[r], total[r]);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < rows)
+  {
+    float most = -INFINITY, all = 0.0f;
+    for (int w = 0; w < kFewThreads / 32; ++w)
+      most = fmaxf(most, parts[w][threadIdx.x].x);
+    const float base = most == -INFINITY ? 0.0f : most;
+    for (int w = 0; w < kFewThreads / 32; ++w)
+      all = fmaf(parts[w][threadIdx.x].y, ex2(parts[w][threadIdx.x].x - base), all);
+    partial[(int64_t)blockIdx.x * rows + threadIdx.x] = make_float2(most, all);
+  }
+}
+
 // lse and loss of every row from the parts.  A block joins `lanes` threads on each of 256 / lanes rows:
 // neighbouring threads read neighbouring rows of a part, and with few rows neighbouring parts.
 __global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restrict__ partial, int64_t parts, int64_t rows,
@@ -699,15 +855,16 @@ __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict_
 
 // out[col] = *factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
+__global__ void __launch_bounds__(1024) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
                                                             int64_t plane, int planes, int64_t rows, int64_t cols,
                                                             const float* __restrict__ factor, T* __restrict__ out)
 {
-  __shared__ float2 parts[8][32];
+  __shared__ float2 parts[32][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t col = (int64_t)blockIdx.x * 64 + 2 * lane; // (ld is a multiple of 256: always inside a row)
   float2 total = make_float2(0.0f, 0.0f);
-  for (int64_t row = warp; row < rows; row += 8)
+#pragma unroll 4
+  for (int64_t row = warp; row < rows; row += 32)
     for (int pl = planes - 1; pl >= 0; --pl)
     {
       const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(slope + pl * plane + row * ld + col));
@@ -718,7 +875,7 @@ __global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16*
   if (warp == 0)
   {
     total = make_float2(0.0f, 0.0f);
-    for (int w = 0; w < 8; ++w)
+    for (int w = 0; w < 32; ++w)
       total.x += parts[w][lane].x, total.y += parts[w][lane].y;
     if (col < cols)
       out[col] = from_float<T>(total.x * *factor);
@@ -770,11 +927,7 @@ int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, 
   P.tiles_m = ceil_div(m, kTile), P.tiles_n = ceil_div(n, COLS);
   P.group_m = std::min<int64_t>(P.tiles_m, 32);
   P.kblocks = (int)ceil_div(contraction, kDepth);
-  // Plane pairs of a pass, smallest terms first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
-  P.passes = planes == 3 ? 6 : 1;
-  P.plane_a = planes == 3 ? 0x001102u : 0u;
-  P.plane_b = planes == 3 ? 0x010120u : 0u;
-  P.splits = (int)std::min<int64_t>(P.splits, (int64_t)P.kblocks * P.passes);
+  P.splits = std::min(P.splits, P.kblocks);
   P.items = P.tiles_m * P.tiles_n * P.splits;
   P.planes = planes;
   auto kernel = vocab_product_kernel<EPI, A_MN, B_MN, COLS>;
@@ -797,7 +950,9 @@ struct Layout
 {
   int pairs = 0, planes = 1, splits = 1;
   bool copy_hidden = false, copy_weight = false;
+  int few = 0;       // blocks of the kernel for few rows
   int64_t share = 0; // columns of a partial sum of exponentials
+  int64_t parts = 0; // partial sums of a row
   int64_t kp = 0;    // columns of the copies
   int64_t ks = 0;    // columns of the sums of d_hidden
   int64_t piece = 0; // vocabulary entries at a time, a multiple of the tile (or all of them)
@@ -830,6 +985,14 @@ int check(const dpc_vocab_ce* c, bool backward, const char* who)
   return DPC_OK;
 }
 
+// Blocks of the kernel for few rows, which are its parts; 0: the tensor cores.
+int few_blocks(const dpc_vocab_ce* c, int sms)
+{
+  if (c->rows > (c->type == DPC_TYPE_F32 ? kFewRows<float> : kFewRows<__nv_bfloat16>) || (size_t)c->rows * ceil_div(c->width, 256) * 256 * sizeof(float) > kFewBytes / 2)
+    return 0;
+  return (int)std::min<int64_t>((c->rows > 4 ? 1 : 2) * sms, ceil_div(c->vocab, kWords * (kFewThreads / 32)));
+}
+
 int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
 {
   int device = 0, sms = 0;
@@ -849,6 +1012,10 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   auto limit = [&](int64_t bytes_each) {
     L.piece = std::min(L.piece, std::max<int64_t>(kTile, (int64_t)(kPieceBytes / bytes_each) / kTile * kTile));
   };
+  if (!backward)
+    L.few = few_blocks(c, sms);
+  if (L.few > 0)
+    L.copy_hidden = L.copy_weight = false;
   if (L.copy_weight)
     limit(L.kp * 2 * L.planes);
   if (backward)
@@ -868,16 +1035,24 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
     L.weight = take((size_t)std::min(L.piece, c->vocab) * L.kp * 2 * L.planes);
   if (backward)
   {
-    // Few tiles of d_hidden: the contraction over the piece is shared out, 4 blocks of it at least each.
-    const int64_t tiles = ceil_div(c->rows, kTile) * (L.ks / (2 * L.share));
-    const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth) * (L.planes == 3 ? 6 : 1);
-    L.splits = (int)std::max<int64_t>(1, std::min(L.pairs / std::max<int64_t>(1, tiles), blocks / 4));
+    // The contraction of d_hidden, over the piece, is shared out where that fills the GPU's last round of tiles (256
+    // tiles on 74 CTA pairs are 4 rounds, in halves 3.5), 4 blocks of it at least each; 3 % a share for its sums.
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(c->rows, kTile) * (L.ks / (2 * L.share)));
+    const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth);
+    double best = 0.0;
+    for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(L.pairs, blocks / 4)); ++n)
+    {
+      const double cost = (double)ceil_div(tiles * n, L.pairs) / n * (1.0 + 0.03 * n);
+      if (n == 1 || cost < best)
+        best = cost, L.splits = (int)n;
+    }
     L.slope = take((size_t)c->rows * L.piece * 2 * L.planes);
     L.sum = take((size_t)L.splits * c->rows * L.ks * sizeof(float));
   }
   else
   {
-    L.partial = take((size_t)(all / L.share) * c->rows * sizeof(float2));
+    L.parts = L.few > 0 ? L.few : round_up(c->vocab, 2 * L.share) / L.share;
+    L.partial = take((size_t)L.parts * c->rows * sizeof(float2));
     L.picked = take((size_t)c->rows * sizeof(float));
   }
   L.bytes = at;
@@ -959,6 +1134,34 @@ GemmParams base_params(const dpc_vocab_ce* c, const Layout& L, int64_t first, ch
   return P;
 }
 
+template <typename T, int ROWS>
+int launch_few(cudaStream_t stream, const dpc_vocab_ce* c, int blocks, float2* partial, float* picked)
+{
+  const size_t bytes = (size_t)ROWS * ceil_div(c->width, 256) * 256 * sizeof(float);
+  const bool wide = reinterpret_cast<uintptr_t>(c->weight) % 16 == 0 && c->weight_stride % (16 / sizeof(T)) == 0 &&
+                    c->width % 8 == 0;
+  auto kernel = wide ? vocab_few_kernel<T, ROWS, true> : vocab_few_kernel<T, ROWS, false>;
+  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  kernel<<<blocks, kFewThreads, bytes, stream>>>(
+      static_cast<const T*>(c->hidden), c->hidden_stride, static_cast<const T*>(c->weight), c->weight_stride,
+      (int)c->rows, (int)c->width, c->vocab, static_cast<const T*>(c->bias), c->scale * kLog2e, c->targets,
+      c->ignore_index, partial, picked);
+  return launched("vocab_few_kernel");
+}
+
+template <typename T>
+int launch_few(cudaStream_t stream, const dpc_vocab_ce* c, int blocks, float2* partial, float* picked)
+{
+  if constexpr (kFewRows<T> > 2)
+  {
+    if (c->rows > 2)
+      return c->rows <= 4 ? launch_few<T, 4>(stream, c, blocks, partial, picked)
+                          : launch_few<T, kFewRows<T>>(stream, c, blocks, partial, picked);
+  }
+  return c->rows == 1 ? launch_few<T, 1>(stream, c, blocks, partial, picked)
+                      : launch_few<T, 2>(stream, c, blocks, partial, picked);
+}
+
 int forward(cudaStream_t stream, const dpc_vocab_ce* c)
 {
   const char* who = "dpc_vocab_ce_forward";
@@ -974,26 +1177,35 @@ int forward(cudaStream_t stream, const dpc_vocab_ce* c)
   if (int rc = workspace_ok(c, L, who))
     return rc;
   char* ws = static_cast<char*>(c->workspace);
-  Operand hidden, weight;
-  if (int rc = prepare_hidden(stream, c, L, false, ws, hidden))
-    return rc;
-  for (int64_t first = 0; first < c->vocab; first += L.piece)
+  float2* partial = reinterpret_cast<float2*>(ws + L.partial);
+  float* picked = reinterpret_cast<float*>(ws + L.picked);
+  if (L.few > 0)
   {
-    const int64_t count = std::min(L.piece, c->vocab - first);
-    if (int rc = piece_weight(stream, c, L, first, count, ws, weight))
-      return rc;
-    GemmParams P = base_params(c, L, first, ws);
-    P.partial = reinterpret_cast<float2*>(ws + L.partial);
-    P.picked = reinterpret_cast<float*>(ws + L.picked);
-    if (int rc = product<EPI_LSE, false, false>(stream, L.pairs, hidden, weight, L.planes, c->rows, count, c->width, P))
+    if (int rc = c->type == DPC_TYPE_F32 ? launch_few<float>(stream, c, L.few, partial, picked)
+                                         : launch_few<__nv_bfloat16>(stream, c, L.few, partial, picked))
       return rc;
   }
+  else
+  {
+    Operand hidden, weight;
+    if (int rc = prepare_hidden(stream, c, L, false, ws, hidden))
+      return rc;
+    for (int64_t first = 0; first < c->vocab; first += L.piece)
+    {
+      const int64_t count = std::min(L.piece, c->vocab - first);
+      if (int rc = piece_weight(stream, c, L, first, count, ws, weight))
+        return rc;
+      GemmParams P = base_params(c, L, first, ws);
+      P.partial = partial, P.picked = picked;
+      if (int rc = product<EPI_LSE, false, false>(stream, L.pairs, hidden, weight, L.planes, c->rows, count, c->width, P))
+        return rc;
+    }
+  }
   int row_shift = 0;
-  while (row_shift < 5 && ((int64_t)1 << row_shift) < c->rows)
+  while (row_shift < 3 && ((int64_t)1 << row_shift) < c->rows)
     ++row_shift;
   vocab_join_kernel<<<(unsigned)ceil_div(c->rows, (int64_t)1 << row_shift), 256, 0, stream>>>(
-      reinterpret_cast<const float2*>(ws + L.partial), round_up(c->vocab, L.planes == 3 ? 128 : kTile) / L.share, c->rows, row_shift,
-      reinterpret_cast<const float*>(ws + L.picked), c->targets, c->vocab, c->ignore_index,
+      partial, L.parts, c->rows, row_shift, picked, c->targets, c->vocab, c->ignore_index,
       c->loss, c->lse);
   return launched("vocab_join_kernel");
 }
@@ -1064,10 +1276,10 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
     {
       const unsigned blocks = (unsigned)ceil_div(count, 64);
       if (c->type == DPC_TYPE_F32)
-        vocab_columns_kernel<float><<<blocks, 256, 0, stream>>>(slope, L.piece, plane, L.planes, c->rows, count,
+        vocab_columns_kernel<float><<<blocks, 1024, 0, stream>>>(slope, L.piece, plane, L.planes, c->rows, count,
                                                                 grad_top, static_cast<float*>(c->d_bias) + first);
       else
-        vocab_columns_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(
+        vocab_columns_kernel<__nv_bfloat16><<<blocks, 1024, 0, stream>>>(
             slope, L.piece, plane, L.planes, c->rows, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
       if (int rc = launched("vocab_columns_kernel"))
         return rc;

@@ -95,6 +95,12 @@ class _Call:
     def empty(self, shape, dtype=None):
         return self.torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
 
+    def like(self, t, dtype=None):
+        """An empty contiguous tensor of t's shape, in the call's type."""
+        if t.is_contiguous():  # (half the time of the general form)
+            return self.torch.empty_like(t) if dtype is None else self.torch.empty_like(t, dtype=dtype)
+        return self.empty(t.shape, dtype)
+
     def run(self, function, *args, workspace=None, call=None):
         """function(stream, *args) on torch's current stream of the tensors' device; ``workspace(call, size)`` tells
         first how much the call needs."""
@@ -143,8 +149,7 @@ def vocab_cross_entropy(hidden, weight, targets, bias=None, *, scale: float = 1.
     call = _Call("vocab_cross_entropy", "hidden", hidden)
     c, targets = _vocab_call(call, hidden, weight, targets, bias, scale, ignore_index)
     lib = _lib.load()
-    loss = call.empty(targets.shape, call.torch.float32)
-    lse = call.empty(targets.shape, call.torch.float32)
+    loss, lse = call.like(targets, call.torch.float32), call.like(targets, call.torch.float32)
     c.loss, c.lse = loss.data_ptr(), lse.data_ptr()
     call.run(lib.dpc_vocab_ce_forward, call=c,
              workspace=lambda size: lib.dpc_vocab_ce_workspace(ctypes.byref(c), 0, ctypes.byref(size)))
@@ -167,8 +172,8 @@ def vocab_cross_entropy_backward(grad_loss, hidden, weight, targets, lse, bias=N
         raise ValueError(f"{call.name}: grad_loss is {tuple(grad_loss.shape)}, {tuple(targets.shape)} or one value is needed")
     one = grad_loss.numel() == 1 or (grad_loss.numel() > 1 and not any(grad_loss.stride()))
     grad_loss, lse = grad_loss if one else grad_loss.contiguous(), lse.contiguous()
-    d_hidden, d_weight = call.empty(hidden.shape), call.empty(weight.shape)
-    d_bias = None if bias is None else call.empty(bias.shape)
+    d_hidden, d_weight = call.like(hidden), call.like(weight)
+    d_bias = None if bias is None else call.like(bias)
     c.lse, c.grad_loss, c.grad_stride = lse.data_ptr(), grad_loss.data_ptr(), 0 if one else 1
     c.d_hidden, c.d_hidden_stride = d_hidden.data_ptr(), c.width
     c.d_weight, c.d_weight_stride = d_weight.data_ptr(), c.width
@@ -240,8 +245,8 @@ def residual_norm(stream, branch=None, *, norm: str = "rms", post_norm: Optional
                    pre_weight, pre_bias, eps)
     lib = _lib.load()
     c.stream = stream.data_ptr()
-    new_stream = stream if branch is None else call.empty(stream.shape)
-    normed = call.empty(stream.shape)
+    new_stream = stream if branch is None else call.like(stream)
+    normed = call.like(stream)
     stats = call.empty((*stream.shape[:-1], 4), call.torch.float32)
     if branch is not None:
         c.new_stream, c.new_stream_stride = new_stream.data_ptr(), c.width
@@ -269,18 +274,18 @@ def residual_norm_backward(d_normed, d_stream, new_stream, branch, stats, *, nor
     if tuple(call.tensor("stats", stats, call.torch.float32).shape) != (*shape[:-1], 4) or not stats.is_contiguous():
         raise ValueError(f"{call.name}: stats has to be the tensor that residual_norm returned")
     c.stats = stats.data_ptr()
-    d_in = call.empty(shape)
+    d_in = call.like(new_stream)
     c.d_stream, c.d_stream_stride = d_in.data_ptr(), width
-    d_branch = None if branch is None else call.empty(shape)
+    d_branch = None if branch is None else call.like(branch)
     if branch is not None:
         c.d_branch, c.d_branch_stride = (d_branch.data_ptr() if c.rows else 16), width
-    d_gate = None if gate is None else call.empty(gate.shape)
+    d_gate = None if gate is None else call.like(gate)
     if gate is not None:
         c.d_gate, c.d_gate_stride = d_gate.data_ptr(), width
     vectors = {}
     for label, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
                      ("pre_bias", pre_bias)):
-        vectors[label] = None if t is None else call.empty(width)
+        vectors[label] = None if t is None else call.like(t)
         if t is not None:
             setattr(c, "d_" + label, vectors[label].data_ptr())
     call.run(lib.dpc_residual_norm_backward, call=c,
@@ -343,8 +348,7 @@ def activate_and_pack(preact, activation):
     if width < 1:
         raise ValueError(f"{call.name}: preact has no columns")
     lib = _lib.load()
-    out = call.empty(preact.shape)
-    codes = call.empty(preact.shape, call.torch.int8)
+    out, codes = call.like(preact), call.like(preact, call.torch.int8)
     scales = call.empty((*preact.shape[:-1], -(-width // BLOCK)), call.torch.float32)
     call.run(lib.dpc_activate_and_pack, call.type, act, rows, width, preact.data_ptr(), stride, out.data_ptr(), width,
              codes.data_ptr(), scales.data_ptr())
@@ -359,7 +363,7 @@ def packed_activation_backward(d_out, packed, activation, *, recompute: bool = F
     if not isinstance(packed, PackedActivations):
         raise TypeError(f"{call.name}: packed is a {type(packed).__name__}, not PackedActivations")
     call.tensor("packed", packed.codes, call.torch.int8)
-    d_preact = call.empty(packed.shape)
-    out = call.empty(packed.shape) if recompute else None
+    d_preact = call.like(d_out)
+    out = call.like(d_out) if recompute else None
     _packed_backward(call, packed, act, d_out, d_preact, out)
     return d_preact, out

@@ -60,7 +60,8 @@ def check_vocab(dp, hidden, weight, targets, bias=None, scale=1.0, ignore_index=
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("rows,width,vocab", [
     (1, 64, 1), (1, 8, 300), (3, 1, 5), (2, 1024, 4099), (127, 96, 257), (128, 64, 256), (129, 65, 255),
-    (257, 72, 1000), (300, 515, 777), (513, 256, 2053), (33, 2048, 600)])
+    (257, 72, 1000), (300, 515, 777), (513, 256, 2053), (33, 2048, 600),
+    (4, 512, 3001), (5, 1000, 1111), (8, 513, 2222), (9, 264, 700)])
 def test_vocab_sizes(dp, rows, width, vocab, kind):
     check_vocab(dp, *vocab_case(rows, width, vocab, TYPES[kind], seed=rows + width))
 
