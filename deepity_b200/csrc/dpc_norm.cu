@@ -16,10 +16,11 @@
 // added by a second kernel in a fixed order: no atomics, the same bits every time.
 //
 // Those sums leave registers for 512 threads an SM, too few to cover the memory's latency with loads of their
-// own: backward fetches its four rows two and more ahead into shared memory by bulk copies.  16384 x 4096 bf16 (805 MB,
-// 123 us at the rate of a copy): 256 us with loads in the threads themselves, 219 with the copies, 168 with arithmetic
-// on pairs and no register spilled; what is left waits for the row's two sums and for weights from L1.  Spills decide
-// here: 100 bytes of them cost 50 us, a second row at once or a warp that only fetches cost more than they gave.
+// own: backward fetches its four rows and their statistics two and more ahead into shared memory by bulk copies.
+// 16384 x 4096 bf16 (805 MB, 123 us at the rate of a copy): 256 us with loads in the threads themselves, 219 with the
+// copies, 160 with arithmetic on pairs and no register spilled; what is left waits for the row's two sums and for
+// weights from L1.  Spills decide here: 100 bytes of them cost 50 us; a second row at once, or a warp that only
+// fetches, cost more than they gave.
 // Forward: 50 us at 16384 x 2048 bf16 (268 MB, 41 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -421,6 +422,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   constexpr bool kAhead = STAGES > 0;
   __shared__ float2 buffer[2][TPR / 32];
   __shared__ uint64_t filled[kUnits][kAhead ? STAGES : 1];
+  __shared__ __align__(16) float4 statistics[kUnits][kAhead ? STAGES : 1];
   __shared__ __align__(16) int give_up[4];
   __shared__ Cursor ahead[kUnits]; // the next row to fetch: kept by thread 0 of a unit, out of the others' registers
   extern __shared__ __align__(128) uint8_t slots[];
@@ -446,13 +448,16 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   if (unit >= P.units)
     return;
   auto fetch = [&](int64_t row, int s) { // by one thread of the unit
-    dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)));
-    auto copy = [&](int k, const void* from, int64_t ld) {
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                       dpc::ptx::smem_u32(slots) + slot_at + (s * kFetched + k) * row_bytes),
-                   "l"(static_cast<const T*>(from) + row * ld), "r"(row_bytes), "r"(dpc::ptx::smem_u32(&full[s]))
+    dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)) + (uint32_t)sizeof(float4));
+    auto bulk = [&](uint32_t to, const void* from, uint32_t bytes) {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                   "l"(from), "r"(bytes), "r"(dpc::ptx::smem_u32(&full[s]))
                    : "memory");
     };
+    auto copy = [&](int k, const void* from, int64_t ld) {
+      bulk(dpc::ptx::smem_u32(slots) + slot_at + (s * kFetched + k) * row_bytes, static_cast<const T*>(from) + row * ld, row_bytes);
+    };
+    bulk(dpc::ptx::smem_u32(&statistics[local][s]), P.stats + row, (uint32_t)sizeof(float4));
     copy(0, P.r, P.r_ld);
     copy(1, P.dh, P.dh_ld);
     if (P.dr)
@@ -475,10 +480,15 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   for (int slot = 0, parity = 0; now.valid(P);)
   {
     const int64_t row = now.row;
-    float4 st = __ldg(P.stats + row);
+    float4 st;
     bool there = true;
     if constexpr (kAhead)
+    {
       there = dpc::ptx::mbar_wait(&full[slot], parity, give_up);
+      st = statistics[local][slot];
+    }
+    else
+      st = __ldg(P.stats + row);
     if (!there) // a copy that is never seen to arrive: NaN
       st = make_float4(NAN, NAN, NAN, NAN);
     auto get = [&](int k, const void* base, int64_t ld, float2x(&v)[M]) {

@@ -70,8 +70,10 @@ struct Tile
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Bytes of slope, and of weight planes, that a piece of the vocabulary may take.
+// Bytes of slope, and of weight planes, that a piece of the vocabulary may take; but 2048 words at least, below
+// which reading and writing the 32-bit sums of d_hidden again for every piece would take as long as its product.
 constexpr size_t kPieceBytes = (size_t)256 << 20;
+constexpr int64_t kPieceLeast = 2048;
 
 enum Epilogue
 {
@@ -1010,7 +1012,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   const int64_t all = round_up(c->vocab, kTile);
   L.piece = all;
   auto limit = [&](int64_t bytes_each) {
-    L.piece = std::min(L.piece, std::max<int64_t>(kTile, (int64_t)(kPieceBytes / bytes_each) / kTile * kTile));
+    L.piece = std::min(L.piece, std::max<int64_t>(kPieceLeast, (int64_t)(kPieceBytes / bytes_each) / kTile * kTile));
   };
   if (!backward)
     L.few = few_blocks(c, sms);

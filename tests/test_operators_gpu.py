@@ -174,6 +174,75 @@ def test_vocab_pieces(dp, rows, width, vocab, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9])
+def test_vocab_few_rows_with_bias_and_ignored_ones(dp, rows, kind):
+    hidden, weight, targets, bias = vocab_case(rows, 200, 2500, TYPES[kind], bias=True, seed=30 + rows, ignore=0.0)
+    check_vocab(dp, hidden, weight, targets, bias, scale=0.5)
+    want = dp.vocab_cross_entropy(hidden, weight, targets, bias)
+    targets[-1] = -100
+    hidden[-1] = float("nan")
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, bias)
+    assert torch.equal(loss[:-1], want[0][:-1]) and torch.equal(lse[:-1], want[1][:-1])
+    assert loss[-1] == 0 and lse[-1] == 0
+
+
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_vocab_every_word_masked(dp, rows):
+    """The sum of no exponentials: its logarithm is -inf, the loss no number; ignored rows stay 0."""
+    hidden, weight, targets, bias = vocab_case(rows, 32, 300, torch.float32, bias=True, seed=31, ignore=0.0)
+    bias.fill_(-float("inf"))
+    if rows > 1:
+        targets[1] = -100
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, bias)
+    counted = targets >= 0
+    assert (lse[counted] == -float("inf")).all() and loss[counted].isnan().all()
+    assert not loss[~counted].any() and not lse[~counted].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [2, 30])
+def test_vocab_large_logits(dp, rows, kind):
+    """Logits of some thousands: exponentials of differences only."""
+    hidden, weight, targets, _ = vocab_case(rows, 64, 600, TYPES[kind], seed=32, ignore=0.0)
+    check_vocab(dp, hidden, weight, targets, scale=1000.0)
+
+
+def test_vocab_unequal_gradients(dp):
+    """Gradients of the losses over many orders of magnitude, zeros and signs among them."""
+    hidden, weight, targets, bias = vocab_case(64, 48, 500, torch.float32, bias=True, seed=33)
+    grad = 10.0 ** torch.linspace(-20, 3, 64, device="cuda") * torch.where(torch.arange(64, device="cuda") % 3 == 0, -1.0, 1.0)
+    grad[10:14] = 0.0
+    check_vocab(dp, hidden, weight, targets, bias, grad=grad)
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, bias)
+    got = dp.vocab_cross_entropy_backward(torch.zeros(64, device="cuda"), hidden, weight, targets, lse, bias)
+    assert not got.hidden.any() and not got.weight.any() and not got.bias.any()
+
+
+def test_vocab_offsets_beyond_32_bits(dp):
+    """A weight of 2^32 elements and more: the last words are read and written where they are."""
+    width, vocab = 8192, (1 << 19) + 65
+    weight = torch.zeros(vocab, width, device="cuda", dtype=torch.bfloat16)
+    g = gen(34)
+    weight[-40:] = normal(g, 40, width, dtype=torch.bfloat16, std=0.05)
+    hidden = normal(g, 3, width, dtype=torch.bfloat16)
+    targets = torch.tensor([vocab - 1, vocab - 30, 5], device="cuda")
+    logits = hidden.double() @ weight[-40:].double().T
+    lse = torch.logsumexp(torch.cat([logits, torch.full((3, 1), float(vocab - 40), device="cuda").double().log()], 1), 1)
+    loss, found = dp.vocab_cross_entropy(hidden, weight, targets)
+    picked = torch.stack([logits[0, 39], logits[1, 10], torch.zeros((), device="cuda").double()])
+    assert (found.double() - lse).abs().max() < 1e-3 and (loss.double() - (lse - picked)).abs().max() < 1e-3
+    got = dp.vocab_cross_entropy_backward(torch.ones(3, device="cuda"), hidden, weight, targets, found)
+    slope = torch.exp(logits - lse[:, None])
+    slope[0, 39] -= 1
+    slope[1, 10] -= 1
+    want = slope.T @ hidden.double()
+    # s and the result rounded to bf16, half a step each, and 1e-3 of lse's error in every probability
+    bound = (2 * 2.0 ** -8 + 2e-3) * (slope.abs().T @ hidden.double().abs()) + 2.0 ** -8 * want.abs()
+    assert ((got.weight[-40:].double() - want).abs() <= bound).all()
+    assert (got.weight[5].double() + hidden[2].double()).abs().max() < 2.0 ** -7 * hidden[2].double().abs().max()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_vocab_no_rows(dp, kind):
     hidden = torch.empty(0, 16, device="cuda", dtype=TYPES[kind])
     weight = normal(gen(0), 30, 16, dtype=TYPES[kind])
@@ -394,6 +463,34 @@ def test_norm_gradient_against_differences(dp):
             h = 2.0 ** -8
             ends = [total(**{**c, name: c[name] + sign * h * step}) for sign in (1, -1)]
             assert abs(float(ends[0] - ends[1]) / (2 * h) - want) < 400 * h * h + 1e-4 / h, (norm, name)
+
+
+def test_norm_and_pack_offsets_beyond_32_bits(dp):
+    """Matrices of more than 2^32 elements: the last row is computed from and written to its place."""
+    rows, width = (1 << 18) + 3, 16384
+    x = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    x[-1] = normal(gen(40), width, dtype=torch.bfloat16)
+    weight = torch.ones(width, device="cuda", dtype=torch.bfloat16)
+    few = dp.residual_norm(x[-1:].clone(), pre_weight=weight)
+    _, normed, stats = dp.residual_norm(x, pre_weight=weight)
+    assert torch.equal(normed[-1:], few[1]) and torch.equal(stats[-1:], few[2]) and not normed[:-1:4099].any()
+    got = dp.residual_norm_backward(normed, None, x, None, stats, pre_weight=weight)
+    want = dp.residual_norm_backward(few[1], None, x[-1:].clone(), None, few[2], pre_weight=weight)
+    assert torch.equal(got.stream[-1:], want.stream) and torch.equal(got.pre_weight, want.pre_weight)
+    del normed, got
+    out, packed = dp.activate_and_pack(x, "gelu")
+    single = dp.activate_and_pack(x[-1:].clone(), "gelu")
+    assert torch.equal(out[-1:], single[0]) and torch.equal(packed.codes[-1:], single[1].codes)
+    assert torch.equal(packed.scales[-1:], single[1].scales)
+    del out
+    d_x, _ = dp.packed_activation_backward(x, packed, "gelu")
+    assert torch.equal(d_x[-1:], dp.packed_activation_backward(x[-1:].clone(), single[1], "gelu")[0])
+
+
+def test_results_carry_no_history(dp):
+    t = {k: v.requires_grad_() if v.is_floating_point() else v for k, v in step_inputs(50).items()}
+    for out in one_step(dp, t):
+        assert not out.requires_grad
 
 
 def test_norm_c_entry_leaves_gaps_and_unwanted_gradients(dp):
