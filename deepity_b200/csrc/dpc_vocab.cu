@@ -51,14 +51,25 @@ constexpr int kTile = 256;       // rows of a pair's tile, and columns but for 3
 constexpr int kRows = 128;       // rows of A that one CTA holds
 constexpr int kDepth = 64;       // contraction depth of a stage: 128 bytes, one swizzle row
 constexpr int kRowBytes = kDepth * 2;
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kRun = 8; // stages whose products the tensor cores add up, where the epilogue warps add the rest
 
+enum Epilogue
+{
+  EPI_LSE,   // maximum and sum of exponentials of a warp's columns of a row
+  EPI_SLOPE, // s of the piece, in bf16 planes
+  EPI_SUM,   // 32-bit sums, added to what earlier pieces left
+  EPI_OUT    // the product itself, in the type of the tensors
+};
+
 // Tiles of COLS columns: each CTA of a pair holds half of B's rows.
-template <int COLS>
+template <int COLS, int EPI>
 struct Tile
 {
+  // 16 warps hide the latency of the exponentials (4096 rows x 64 against 50021 words: 124 -> 104 us, x 512: 156 -> 136); where they
+  // also convert and store, or hold sums in registers, their 96 registers cost more (79 -> 89 us a piece of 25088).
+  static constexpr int kEpilogueWarps = COLS == 256 && EPI == EPI_LSE ? 16 : 8;
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+
   static constexpr bool kRuns = COLS < kTile;
   static constexpr int kPlanes = kRuns ? 3 : 1; // of each operand, in a stage
   static constexpr int kABytes = kRows * kRowBytes, kBBytes = COLS / 2 * kRowBytes;
@@ -66,7 +77,7 @@ struct Tile
   static constexpr int kStages = kRuns ? 3 : 6;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
   static constexpr int kSets = kRuns ? 2 : 1; // accumulators of a tile: hi x hi, and the five smaller products
-  static constexpr int kShare = COLS / 2;     // columns of an epilogue warp
+  static constexpr int kShare = COLS / (kEpilogueWarps / 4); // columns of an epilogue warp
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -75,17 +86,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr size_t kPieceBytes = (size_t)256 << 20;
 constexpr int64_t kPieceLeast = 2048;
 
-enum Epilogue
-{
-  EPI_LSE,   // maximum and sum of exponentials of half a tile of a row
-  EPI_SLOPE, // s of the piece, in bf16 planes
-  EPI_SUM,   // 32-bit sums, added to what earlier pieces left
-  EPI_OUT    // the product itself, in the type of the tensors
-};
-
 struct GemmParams
 {
-  int64_t tiles_m, tiles_n, group_m, items; // items = splits * tiles_m * tiles_n
+  // (32 bits: divisions of 64 took longer than a tile's product where the rows are short)
+  uint32_t tiles_m, tiles_n, tiles, group_m, items; // tiles = tiles_m * tiles_n, items = splits * tiles
   int splits, kblocks;
   int64_t m, n;              // rows and columns of the product
   // logits
@@ -95,7 +99,7 @@ struct GemmParams
   const int64_t* targets;
   int64_t vocab, first; // first: vocabulary entry of column 0
   int64_t ignore_index;
-  float2* partial; // EPI_LSE: [block of the vocabulary, half a tile wide][row]
+  float2* partial; // EPI_LSE: [block of the vocabulary, a warp's columns wide][row]
   float* picked;   // EPI_LSE: logit of the target, in units of log 2
   const float* lse;
   const float* grad;
@@ -104,7 +108,6 @@ struct GemmParams
   float scale;
   __nv_bfloat16* slope;
   int64_t slope_ld, slope_plane;
-  int planes;
   float* sum; // EPI_SUM
   int64_t sum_ld, sum_split;
   int add;
@@ -125,22 +128,61 @@ __device__ __forceinline__ bool counted(int64_t target, int64_t vocab, int64_t i
   return target >= 0 && target < vocab && target != ignore_index;
 }
 
+// A warp has read its accumulators: their next tile may be multiplied.  Relaxed: what was read is in registers, and
+// a release would wait for the epilogue's stores as well.
+__device__ __forceinline__ void accumulators_read(uint32_t bar, int lane)
+{
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0)
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// 32 columns of tensor memory on their way into registers; tmem_wait ends the wait for them (the registers pass
+// through it, so that nothing reads them before).
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32])
+{
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+               "[%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                 "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                 "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32])
+{
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 // Which tile a work item is: the tiles of `group_m` row blocks go down the rows first, so that the
 // CTA pairs at work share a few column blocks (weights, read once) and the rows of the group stay in L2.
-__device__ __forceinline__ void locate(const GemmParams& P, int64_t item, int& split, int64_t& tm, int64_t& tn)
+__device__ __forceinline__ void locate(const GemmParams& P, uint32_t item, int& split, uint32_t& tm, uint32_t& tn)
 {
-  const int64_t tiles = P.tiles_m * P.tiles_n;
-  split = (int)(item / tiles);
-  const int64_t tile = item - split * tiles, group = tile / (P.group_m * P.tiles_n);
-  const int64_t first = group * P.group_m, rest = tile - first * P.tiles_n;
-  const int64_t height = P.tiles_m - first < P.group_m ? P.tiles_m - first : P.group_m;
+  split = P.splits == 1 ? 0 : (int)(item / P.tiles);
+  const uint32_t tile = item - split * P.tiles;
+  const uint32_t group = P.tiles_m == P.group_m ? 0 : tile / (P.group_m * P.tiles_n);
+  const uint32_t first = group * P.group_m, rest = tile - first * P.tiles_n;
+  const uint32_t height = min(P.tiles_m - first, P.group_m);
   tn = rest / height;
   tm = first + rest - tn * height;
 }
 
 __device__ __forceinline__ void range_of(const GemmParams& P, int split, int& begin, int& end)
 {
-  begin = (int)((int64_t)P.kblocks * split / P.splits), end = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
+  begin = 0, end = P.kblocks;
+  if (P.splits > 1)
+    begin = (int)((int64_t)P.kblocks * split / P.splits), end = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
 }
 
 // 32 logits of a row in units of log 2, -inf outside the vocabulary.
@@ -173,11 +215,11 @@ __device__ __forceinline__ void logits32(const GemmParams& P, int64_t col, float
 }
 
 template <int EPI, bool A_MN, bool B_MN, int COLS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kThreads, 1)
     vocab_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const GemmParams P)
 {
-  using C = Tile<COLS>;
+  using C = Tile<COLS, EPI>;
   constexpr int kStages = C::kStages, kStageBytes = C::kStageBytes;
   constexpr uint32_t kTmemColumns = 2 * C::kSets * COLS;
   constexpr uint32_t kInstr = (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
@@ -196,7 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int64_t begin = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint32_t begin = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (threadIdx.x == 0)
   {
@@ -208,7 +250,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int a = 0; a < 2; ++a)
     {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 2 * kEpilogueWarps); // both CTAs' epilogue warps arrive on the leader's
+      mbar_init(&tempty[a], 2 * C::kEpilogueWarps); // both CTAs' epilogue warps arrive on the leader's
     }
     *abort_flag = 0;
     *reinterpret_cast<volatile long long*>(abort_flag + 2) = kWaitCyclesDefault;
@@ -239,10 +281,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int s = 0;
       uint32_t phase = 1;
       bool alive = true;
-      for (int64_t item = begin; item < P.items && alive; item += step)
+      for (uint32_t item = begin; item < P.items && alive; item += step)
       {
         int split, it, it_end;
-        int64_t tm, tn;
+        uint32_t tm, tn;
         locate(P, item, split, tm, tn);
         range_of(P, split, it, it_end);
         const int m0 = (int)(tm * kTile) + (int)rank * kRows, n0 = (int)(tn * COLS) + (int)rank * (COLS / 2);
@@ -300,10 +342,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int s = 0, turn = 0;
       uint32_t phase = 0;
       bool alive = true;
-      for (int64_t item = begin; item < P.items && alive; item += step)
+      for (uint32_t item = begin; item < P.items && alive; item += step)
       {
         int it, it_end;
-        range_of(P, (int)(item / (P.tiles_m * P.tiles_n)), it, it_end);
+        range_of(P, P.splits == 1 ? 0 : (int)(item / P.tiles), it, it_end);
         while (it < it_end && alive)
         {
           const int run_end = C::kRuns && it + kRun < it_end ? it + kRun : it_end;
@@ -357,32 +399,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   else if (warp >= 4)
   {
-    // ---------------------------------------------------------------- epilogue: a row a lane, half a tile's columns a warp
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    // ---------------------------------------------------------------- epilogue: a row a lane, kShare columns a warp
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
     int turn = 0;
     bool alive = true; // a wait gave up: everything from then on is NaN
-    for (int64_t item = begin; item < P.items; item += step)
+    for (uint32_t item = begin; item < P.items; item += step)
     {
       int split;
-      int64_t tm, tn;
+      uint32_t tm, tn;
       locate(P, item, split, tm, tn);
-      const int64_t row = tm * kTile + rank * kRows + quarter * 32 + lane;
-      const int64_t col0 = tn * COLS + half * C::kShare;
+      const int64_t row = (int64_t)tm * kTile + rank * kRows + quarter * 32 + lane;
+      const int64_t col0 = (int64_t)tn * COLS + part * C::kShare;
       const bool inside = row < P.m;
       int64_t target = -1; // column of the target, outside the tile: not this one
       bool count = false;
       float lse2 = 0.0f, slope_scale = 0.0f;
       if ((EPI == EPI_LSE || EPI == EPI_SLOPE) && inside)
       {
-        const int64_t t = P.targets[row];
+        const int64_t t = __ldg(P.targets + row);
+        if (EPI == EPI_SLOPE) // (of rows that do not count as well: the loads go out together)
+        {
+          lse2 = __ldg(P.lse + row) * kLog2e;
+          slope_scale = __fdiv_rn(__ldg(P.grad + row * P.grad_stride), __ldg(P.grad_top));
+        }
         count = counted(t, P.vocab, P.ignore_index);
         if (count)
           target = t - P.first;
-        if (EPI == EPI_SLOPE && count)
-        {
-          lse2 = P.lse[row] * kLog2e;
-          slope_scale = __fdiv_rn(P.grad[row * P.grad_stride], *P.grad_top);
-        }
       }
       int it, it_end;
       range_of(P, split, it, it_end);
@@ -400,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + half * C::kShare;
+          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + part * C::kShare;
 #pragma unroll
           for (int c = 0; c < C::kShare / 32; ++c)
           {
@@ -415,10 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i)
               sums[C::kRuns ? c : 0][i] += v[i];
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0)
-            mbar_arrive_cluster(lead_tempty + (uint32_t)(acc * 8));
+          accumulators_read(lead_tempty + (uint32_t)(acc * 8), lane);
         }
       }
       const int acc = turn & 1;
@@ -426,69 +465,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         alive = __all_sync(0xffffffffu, mbar_wait_cluster(&tfull[acc], (turn >> 1) & 1, abort_flag));
       ++turn;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + half * C::kShare;
-      const float out_factor = EPI == EPI_OUT ? *P.grad_top * P.scale : 1.0f;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + part * C::kShare;
+      if ((EPI == EPI_LSE || EPI == EPI_SLOPE) && item + step < P.items)
+      {
+        // the next tile's targets come into L1 while this one is worked on
+        int s;
+        uint32_t m, n;
+        locate(P, item + step, s, m, n);
+        const int64_t next = (int64_t)m * kTile + rank * kRows + quarter * 32 + lane;
+        if (next < P.m)
+        {
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(P.targets + next));
+          if (EPI == EPI_SLOPE)
+          {
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(P.lse + next));
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(P.grad + next * P.grad_stride));
+          }
+        }
+      }
+      const float out_factor = EPI == EPI_OUT ? __ldg(P.grad_top) * P.scale : 1.0f;
       float top = -INFINITY, total = 0.0f;
-#pragma unroll(C::kRuns ? C::kShare / 32 : 1)
+      uint32_t raw[C::kRuns ? 1 : 2][32];
+      __syncwarp();
+      if (!C::kRuns)
+        tmem_load(taddr, raw[0]); // (whatever is there, after a wait that gave up)
+#pragma unroll
       for (int c = 0; c < C::kShare / 32; ++c)
       {
         const int64_t col = col0 + 32 * c;
         float v[32];
         __syncwarp();
-        tc_ld32(taddr + 32 * c, v); // (a read of whatever is there, after a wait that gave up)
         if (C::kRuns)
         {
           float w[32];
+          tc_ld32(taddr + 32 * c, v);
           tc_ld32(taddr + COLS + 32 * c, w);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             v[i] += several ? sums[C::kRuns ? c : 0][i] + w[i] : w[i];
         }
+        else
+        {
+          // the next columns come while these are worked on
+          uint32_t(&now)[32] = raw[C::kRuns ? 0 : c & 1];
+          tmem_wait(now);
+          if (c + 1 < C::kShare / 32)
+            tmem_load(taddr + 32 * (c + 1), raw[C::kRuns ? 0 : (c + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = __uint_as_float(now[i]);
+        }
+        if (c + 1 == C::kShare / 32)
+          accumulators_read(lead_tempty + (uint32_t)(acc * 8), lane);
         if (!alive)
         {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             v[i] = NAN;
         }
-        if (EPI == EPI_LSE)
+        // logits are factor * v, in units of log 2
+        float factor = P.factor;
+        if ((EPI == EPI_LSE || EPI == EPI_SLOPE) && (P.bias || col + 32 > P.n))
         {
           logits32(P, col, v);
-          if (target >= col && target < col + 32)
+          factor = 1.0f;
+        }
+        const int hot = target >= col && target < col + 32 ? (int)(target - col) : -1;
+        if (EPI == EPI_LSE)
+        {
+          if (hot >= 0)
           {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (target == col + i)
-                P.picked[row] = v[i];
+              if (i == hot)
+                P.picked[row] = v[i] * factor;
           }
-          float most = v[0];
+          float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int i = 1; i < 32; ++i)
-            most = fmaxf(most, v[i]);
-          most = fmaxf(most, top);
+          for (int i = 4; i < 32; ++i)
+            most[i & 3] = fmaxf(most[i & 3], v[i]);
+          const float high = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * factor, top);
           // (nothing but -inf so far: zero in its place leaves the sum at 0, or NaN where a logit is NaN)
-          const float base = most == -INFINITY ? 0.0f : most;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float base = high == -INFINITY ? 0.0f : high;
+          float2x sum[2] = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            sum[i & 3] += ex2(v[i] - base);
-          total = fmaf(total, ex2(top - base), (sum[0] + sum[1]) + (sum[2] + sum[3]));
-          top = most;
+          for (int i = 0; i < 32; i += 2)
+          {
+            const float2 e = halves(fma2(pair(v[i], v[i + 1]), pair(factor), pair(-base)));
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(ex2(e.x), ex2(e.y)));
+          }
+          const float2 all = halves(add2(sum[0], sum[1]));
+          total = fmaf(total, ex2(top - base), all.x + all.y);
+          top = high;
         }
         else if (EPI == EPI_SLOPE)
         {
-          logits32(P, col, v);
-          const int hot = target >= col && target < col + 32 ? (int)(target - col) : -1;
           // (past the last column of the piece: exp(-inf) = 0 is written, and nothing reads it)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 32; i += 2)
           {
-            const float p = ex2(v[i] - lse2) - (i == hot ? 1.0f : 0.0f);
-            v[i] = count ? slope_scale * p : 0.0f; // an ignored row is 0 whatever it holds
+            const float2 e = halves(fma2(pair(v[i], v[i + 1]), pair(factor), pair(-lse2)));
+            v[i] = ex2(e.x), v[i + 1] = ex2(e.y);
           }
+          if (hot >= 0)
+          {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[i] -= i == hot ? 1.0f : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = count ? slope_scale * v[i] : 0.0f; // an ignored row is 0 whatever it holds
           if (inside)
           {
             __nv_bfloat16* dst = P.slope + row * P.slope_ld + col;
-            for (int pl = 0; pl < P.planes; ++pl, dst += P.slope_plane)
+#pragma unroll
+            for (int pl = 0; pl < C::kPlanes; ++pl, dst += P.slope_plane)
             {
               float w[16];
 #pragma unroll
@@ -561,10 +653,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive_cluster(lead_tempty + (uint32_t)(acc * 8));
       if (EPI == EPI_LSE && inside)
         P.partial[((P.first + col0) / C::kShare) * P.m + row] = make_float2(top, total);
     }
@@ -858,7 +946,7 @@ __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict_
 // out[col] = *factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(1024) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
-                                                            int64_t plane, int planes, int64_t rows, int64_t cols,
+                                                            int64_t plane, int64_t rows, int64_t cols,
                                                             const float* __restrict__ factor, T* __restrict__ out)
 {
   __shared__ float2 parts[32][32];
@@ -867,7 +955,8 @@ __global__ void __launch_bounds__(1024) vocab_columns_kernel(const __nv_bfloat16
   float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll 4
   for (int64_t row = warp; row < rows; row += 32)
-    for (int pl = planes - 1; pl >= 0; --pl)
+#pragma unroll
+    for (int pl = sizeof(T) == 4 ? 2 : 0; pl >= 0; --pl)
     {
       const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(slope + pl * plane + row * ld + col));
       total.x += v.x, total.y += v.y;
@@ -919,23 +1008,25 @@ template <int EPI, bool A_MN, bool B_MN, int COLS>
 int product(cudaStream_t stream, int pairs, const Operand& a, const Operand& b, int planes, int64_t m, int64_t n,
             int64_t contraction, GemmParams P)
 {
-  using C = Tile<COLS>;
+  using C = Tile<COLS, EPI>;
   CUtensorMap map_a, map_b;
   if (int rc = operand_map(&map_a, a.base, a.cols, a.rows, a.ld, planes, a.plane, A_MN ? kDepth : kRows))
     return rc;
   if (int rc = operand_map(&map_b, b.base, b.cols, b.rows, b.ld, planes, b.plane, B_MN ? kDepth : COLS / 2))
     return rc;
   P.m = m, P.n = n;
-  P.tiles_m = ceil_div(m, kTile), P.tiles_n = ceil_div(n, COLS);
-  P.group_m = std::min<int64_t>(P.tiles_m, 32);
   P.kblocks = (int)ceil_div(contraction, kDepth);
   P.splits = std::min(P.splits, P.kblocks);
-  P.items = P.tiles_m * P.tiles_n * P.splits;
-  P.planes = planes;
+  const int64_t tiles_m = ceil_div(m, kTile), tiles_n = ceil_div(n, COLS);
+  if (tiles_m * tiles_n > ((int64_t)1 << 30) / P.splits)
+    return dpc::fail(DPC_ERR_TOO_LARGE, "vocabulary loss: more than 2^30 tiles of 256 rows and 128 or 256 columns");
+  P.tiles_m = (uint32_t)tiles_m, P.tiles_n = (uint32_t)tiles_n, P.tiles = P.tiles_m * P.tiles_n;
+  P.group_m = std::min<uint32_t>(P.tiles_m, 32);
+  P.items = P.tiles * P.splits;
   auto kernel = vocab_product_kernel<EPI, A_MN, B_MN, COLS>;
   DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
   const int blocks = 2 * (int)std::min<int64_t>(P.items, pairs);
-  kernel<<<blocks, kThreads, C::kSmemBytes, stream>>>(map_a, map_b, P);
+  kernel<<<blocks, C::kThreads, C::kSmemBytes, stream>>>(map_a, map_b, P);
   return launched("vocab_product_kernel");
 }
 
@@ -953,6 +1044,7 @@ struct Layout
   int pairs = 0, planes = 1, splits = 1;
   bool copy_hidden = false, copy_weight = false;
   int few = 0;       // blocks of the kernel for few rows
+  int64_t cols = 0;  // columns of a tile
   int64_t share = 0; // columns of a partial sum of exponentials
   int64_t parts = 0; // partial sums of a row
   int64_t kp = 0;    // columns of the copies
@@ -1006,7 +1098,8 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   // does not reach d_weight as 0 * inf)
   L.copy_hidden = backward || L.planes > 1 || !tma_ready(c->hidden, c->hidden_stride);
   L.copy_weight = L.planes > 1 || !tma_ready(c->weight, c->weight_stride);
-  L.share = L.planes == 3 ? Tile<128>::kShare : Tile<256>::kShare;
+  L.cols = L.planes == 3 ? 128 : kTile;
+  L.share = L.planes == 3 ? Tile<128, EPI_LSE>::kShare : Tile<256, EPI_LSE>::kShare;
   L.kp = round_up(c->width, 8);
   L.ks = round_up(c->width, kTile);
   const int64_t all = round_up(c->vocab, kTile);
@@ -1039,7 +1132,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   {
     // The contraction of d_hidden, over the piece, is shared out where that fills the GPU's last round of tiles (256
     // tiles on 74 CTA pairs are 4 rounds, in halves 3.5), 4 blocks of it at least each; 3 % a share for its sums.
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(c->rows, kTile) * (L.ks / (2 * L.share)));
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(c->rows, kTile) * (L.ks / L.cols));
     const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth);
     double best = 0.0;
     for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(L.pairs, blocks / 4)); ++n)
@@ -1053,7 +1146,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   }
   else
   {
-    L.parts = L.few > 0 ? L.few : round_up(c->vocab, 2 * L.share) / L.share;
+    L.parts = L.few > 0 ? L.few : round_up(c->vocab, L.cols) / L.share;
     L.partial = take((size_t)L.parts * c->rows * sizeof(float2));
     L.picked = take((size_t)c->rows * sizeof(float));
   }
@@ -1278,11 +1371,11 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
     {
       const unsigned blocks = (unsigned)ceil_div(count, 64);
       if (c->type == DPC_TYPE_F32)
-        vocab_columns_kernel<float><<<blocks, 1024, 0, stream>>>(slope, L.piece, plane, L.planes, c->rows, count,
+        vocab_columns_kernel<float><<<blocks, 1024, 0, stream>>>(slope, L.piece, plane, c->rows, count,
                                                                 grad_top, static_cast<float*>(c->d_bias) + first);
       else
         vocab_columns_kernel<__nv_bfloat16><<<blocks, 1024, 0, stream>>>(
-            slope, L.piece, plane, L.planes, c->rows, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
+            slope, L.piece, plane, c->rows, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
       if (int rc = launched("vocab_columns_kernel"))
         return rc;
     }
