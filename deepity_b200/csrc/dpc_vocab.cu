@@ -976,36 +976,55 @@ __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict_
   }
 }
 
-// out[col] = *factor * sum over the rows and planes of slope, 64 columns a block, rows in a fixed order.
-template <typename T>
-__global__ void __launch_bounds__(1024) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
-                                                            int64_t plane, int64_t rows, int64_t cols,
-                                                            const float* __restrict__ factor, T* __restrict__ out)
+// sums[part][col] = sum of slope over the planes and a part of the rows: 256 columns and a part a block, 8 columns a
+// lane, rows in a fixed order.  (With 64 columns and all rows a block the loads under way were too few: 32 us where
+// this and the kernel below take 15, for 777 rows of 10007 in three planes.)
+constexpr int kColumnParts = 16;
+
+template <int PLANES>
+__global__ void __launch_bounds__(256) vocab_columns_kernel(const __nv_bfloat16* __restrict__ slope, int64_t ld,
+                                                           int64_t plane, int64_t rows, float* __restrict__ sums)
 {
-  __shared__ float2 parts[32][32];
+  __shared__ float parts[8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t col = (int64_t)blockIdx.x * 64 + 2 * lane; // (ld is a multiple of 256: always inside a row)
-  float2 total = make_float2(0.0f, 0.0f);
+  const int64_t col = (int64_t)blockIdx.x * 256 + 8 * lane; // (ld is a multiple of 256: always inside a row)
+  const int64_t begin = rows * blockIdx.y / gridDim.y, end = rows * (blockIdx.y + 1) / gridDim.y;
+  float total[8] = {};
 #pragma unroll 4
-  for (int64_t row = warp; row < rows; row += 32)
+  for (int64_t row = begin + warp; row < end; row += 8)
 #pragma unroll
-    for (int pl = sizeof(T) == 4 ? 2 : 0; pl >= 0; --pl)
+    for (int pl = PLANES - 1; pl >= 0; --pl)
     {
-      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(slope + pl * plane + row * ld + col));
-      total.x += v.x, total.y += v.y;
+      float v[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(slope + pl * plane + row * ld + col)), v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        total[i] += v[i];
     }
-  parts[warp][lane] = total;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    parts[warp][8 * lane + i] = total[i];
   __syncthreads();
-  if (warp == 0)
-  {
-    total = make_float2(0.0f, 0.0f);
-    for (int w = 0; w < 32; ++w)
-      total.x += parts[w][lane].x, total.y += parts[w][lane].y;
-    if (col < cols)
-      out[col] = from_float<T>(total.x * *factor);
-    if (col + 1 < cols)
-      out[col + 1] = from_float<T>(total.y * *factor);
-  }
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w)
+    s += parts[w][threadIdx.x];
+  sums[blockIdx.y * ld + (int64_t)blockIdx.x * 256 + threadIdx.x] = s;
+}
+
+// out[col] = *factor * the sum of the parts
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_columns_join_kernel(const float* __restrict__ sums, int64_t ld, int parts,
+                                                                int64_t cols, const float* __restrict__ factor,
+                                                                T* __restrict__ out)
+{
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col >= cols)
+    return;
+  float s = 0.0f;
+  for (int p = 0; p < parts; ++p)
+    s += sums[p * ld + col];
+  out[col] = from_float<T>(s * *factor);
 }
 
 // ------------------------------------------------------------------------------ host
@@ -1083,7 +1102,8 @@ struct Layout
   int64_t kp = 0;    // columns of the copies
   int64_t ks = 0;    // columns of the sums of d_hidden
   int64_t piece = 0; // vocabulary entries at a time, a multiple of the tile (or all of them)
-  size_t grad_top = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
+  int column_parts = 1; // of the rows, in the sums of a bias gradient
+  size_t grad_top = 0, columns = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
 };
 
 bool tma_ready(const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
@@ -1176,6 +1196,9 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
     }
     L.slope = take((size_t)c->rows * L.piece * 2 * L.planes);
     L.sum = take((size_t)L.splits * c->rows * L.ks * sizeof(float));
+    L.column_parts = (int)std::min<int64_t>(kColumnParts, ceil_div(c->rows, 64));
+    if (c->bias)
+      L.columns = take((size_t)L.column_parts * L.piece * sizeof(float));
   }
   else
   {
@@ -1402,13 +1425,21 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
       return rc;
     if (c->d_bias)
     {
-      const unsigned blocks = (unsigned)ceil_div(count, 64);
+      float* columns = reinterpret_cast<float*>(ws + L.columns);
+      const unsigned blocks = (unsigned)ceil_div(count, 256);
+      const dim3 grid(blocks, (unsigned)L.column_parts);
       if (c->type == DPC_TYPE_F32)
-        vocab_columns_kernel<float><<<blocks, 1024, 0, stream>>>(slope, L.piece, plane, c->rows, count,
-                                                                grad_top, static_cast<float*>(c->d_bias) + first);
+      {
+        vocab_columns_kernel<3><<<grid, 256, 0, stream>>>(slope, L.piece, plane, c->rows, columns);
+        vocab_columns_join_kernel<float><<<blocks, 256, 0, stream>>>(columns, L.piece, L.column_parts, count, grad_top,
+                                                                    static_cast<float*>(c->d_bias) + first);
+      }
       else
-        vocab_columns_kernel<__nv_bfloat16><<<blocks, 1024, 0, stream>>>(
-            slope, L.piece, plane, c->rows, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
+      {
+        vocab_columns_kernel<1><<<grid, 256, 0, stream>>>(slope, L.piece, plane, c->rows, columns);
+        vocab_columns_join_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(
+            columns, L.piece, L.column_parts, count, grad_top, static_cast<__nv_bfloat16*>(c->d_bias) + first);
+      }
       if (int rc = launched("vocab_columns_kernel"))
         return rc;
     }
