@@ -9,7 +9,7 @@
 // twice; a thread reads its next part before it works on this one, in 32-byte accesses.  The code is x * (127 / max)
 // rounded to even: one division a block instead of one an element, and a product whose rounding is that of 32-bit
 // arithmetic everywhere.  16384 x 8192 bf16, gelu: forward 116 us (671 MB, 103 us at the rate of a copy), backward
-// with f(x) 149 us (940 MB, 144), values alone 83 us (403 MB, 62).  16-byte accesses and conversions by the conversion
+// with f(x) 149 us (940 MB, 144), values alone 67 us (403 MB, 62).  16-byte accesses and conversions by the conversion
 // unit: 187, 231 and 107.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -296,8 +296,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
   }
 }
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 3)
+// SLOPE: d_preact (and out where it is wanted); otherwise out alone, with fewer registers and so more loads under way.
+template <typename T, bool WIDE, bool SLOPE>
+__global__ void __launch_bounds__(kThreads, SLOPE ? 3 : 5)
     packed_backward_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t rows, int64_t width,
                            int64_t blocks, int act, const T* __restrict__ d_out, int64_t d_out_ld,
                            T* __restrict__ d_preact, int64_t d_preact_ld, T* __restrict__ out, int64_t out_ld)
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     const int64_t first = at.block * kBlock;
     const int8_t* from = codes + at.row * width;
     next_scale = __ldg(scales + at.row * blocks + at.block);
-    if (d_out)
+    if (SLOPE)
       next.fetch(d_out + at.row * d_out_ld, first, part, width);
     if constexpr (WIDE)
     {
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         const float2 w = halves(mul2(add2(x, pair(-8388736.0f)), pair(scale)));
         v[i] = w.x, v[i + 1] = w.y;
       }
-      if (d_out)
+      if constexpr (SLOPE)
       {
         float g[N];
         now.get(h, g);
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         result.set(h, f);
       }
     }
-    if (d_out)
+    if (SLOPE)
       slope.store(d_preact + row * d_preact_ld, first, part, width);
     if (out)
       result.store(out + row * out_ld, first, part, width);
@@ -444,10 +445,9 @@ void launch_backward(cudaStream_t stream, bool w, int act, int64_t rows, int64_t
   const unsigned grid = w ? grid_for<true>(rows * blocks) : grid_for<false>(rows * blocks);
   const T* g = static_cast<const T*>(d_out);
   T *dx = static_cast<T*>(d_preact), *to = static_cast<T*>(out);
-  if (w)
-    packed_backward_kernel<T, true><<<grid, kThreads, 0, stream>>>(codes, scales, rows, width, blocks, act, g, d_out_ld, dx, d_preact_ld, to, out_ld);
-  else
-    packed_backward_kernel<T, false><<<grid, kThreads, 0, stream>>>(codes, scales, rows, width, blocks, act, g, d_out_ld, dx, d_preact_ld, to, out_ld);
+  auto kernel = w ? (g ? packed_backward_kernel<T, true, true> : packed_backward_kernel<T, true, false>)
+                  : (g ? packed_backward_kernel<T, false, true> : packed_backward_kernel<T, false, false>);
+  kernel<<<grid, kThreads, 0, stream>>>(codes, scales, rows, width, blocks, act, g, d_out_ld, dx, d_preact_ld, to, out_ld);
 }
 } // namespace
 

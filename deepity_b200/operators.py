@@ -40,14 +40,14 @@ def _stream(torch, device):
 class _Call:
     """What the tensors of one call have in common: type and device, taken from the first.  (Few and cheap
     steps: a call for one token is bound by the host.)"""
-    __slots__ = ("torch", "name", "dtype", "device", "type")
+    __slots__ = ("torch", "name", "first", "dtype", "device", "type")
 
     def __init__(self, name, first_name, first):
         torch = self.torch = _torch()
         self.name = name
         if not isinstance(first, torch.Tensor):
             raise TypeError(f"{name}: {first_name} has to be a torch tensor, not {type(first).__name__}")
-        self.dtype, self.device = first.dtype, first.device
+        self.first, self.dtype, self.device = first, first.dtype, first.device
         if self.dtype is torch.bfloat16:
             self.type = 1
         elif self.dtype is torch.float32:
@@ -93,7 +93,7 @@ class _Call:
         return t.data_ptr()
 
     def empty(self, shape, dtype=None):
-        return self.torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
+        return self.first.new_empty(shape, dtype=dtype or self.dtype)
 
     def like(self, t, dtype=None):
         """An empty contiguous tensor of t's shape, in the call's type."""

@@ -693,7 +693,7 @@ DPC_API int dpc_vocab_ce_backward(void* stream, const dpc_vocab_ce* call);
  * stats [rows, 4]: mean and 1/deviation of the branch (0, 0 without post_norm), of the new stream (before it is rounded).
  * Backward reads new_stream, branch and stats: d_normed and d_new_stream (NULL: none) are the gradients
  * of the two outputs; d_branch, d_gate and the gradients of weights and biases are written where the
- * tensor is given (a gradient pointer may be NULL: not wanted).  width 16384 at most; rows may be 0 (vector gradients are
+ * tensor is given (a gradient pointer may be NULL: not wanted).  width 16384 at most, rows below 2^31; rows may be 0 (vector gradients are
  * then zeros).  The workspace depends on pointers and strides too: ask with those of the call. */
 typedef enum dpc_norm
 {
