@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) norm_join_kernel(const JoinPa
 int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
 // Threads of a row.  Two vectors of 8 a thread, four in the widest rows; one, as far as 512 threads go, in backward
-// passes that keep sums of biases or load element by element (`lean`): two would not fit their registers.
+// passes that keep sums of biases or load element by element (`lean`; two would not fit their registers) and in those of
+// 32-bit rows (with two, the rows of an SM's blocks would not fit its shared memory two ahead).
 int threads_of(int64_t width, bool lean)
 {
   const int64_t each = lean ? 8 : 16;
@@ -868,7 +869,7 @@ int dispatch_forward(cudaStream_t stream, const NormParams& P)
 template <typename T, bool WIDE, bool BIAS>
 int dispatch_backward(cudaStream_t stream, const NormParams& P)
 {
-  constexpr bool kLean = BIAS || !WIDE;
+  constexpr bool kLean = BIAS || !WIDE || sizeof(T) == 4;
   constexpr int VPT = kLean ? 1 : 2;
   switch (threads_of(P.width, kLean))
   {
@@ -910,6 +911,8 @@ bool wide_backward(const dpc_residual_norm* c)
 }
 
 bool with_bias(const dpc_residual_norm* c) { return c->d_post_bias || c->d_pre_bias; }
+
+bool lean_backward(const dpc_residual_norm* c, bool is_wide) { return with_bias(c) || !is_wide || c->type == DPC_TYPE_F32; }
 
 int forward(cudaStream_t stream, const dpc_residual_norm* c)
 {
@@ -962,7 +965,7 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
     return rc;
   const bool w = wide_backward(c);
   Split S;
-  if (int rc = split_rows(c, with_bias(c) || !w, S))
+  if (int rc = split_rows(c, lean_backward(c, w), S))
     return rc;
   if (!c->workspace || reinterpret_cast<uintptr_t>(c->workspace) % 256 || c->workspace_bytes < S.bytes)
     return dpc::fail(DPC_ERR_INVALID, who + ": " + std::to_string(S.bytes) +
@@ -1005,7 +1008,7 @@ int dpc_residual_norm_workspace(const dpc_residual_norm* c, size_t* bytes)
     if (int rc = check(c, "dpc_residual_norm_workspace"))
       return rc;
     Split S;
-    if (int rc = split_rows(c, with_bias(c) || !wide_backward(c), S))
+    if (int rc = split_rows(c, lean_backward(c, wide_backward(c)), S))
       return rc;
     *bytes = S.bytes;
     return (int)DPC_OK;

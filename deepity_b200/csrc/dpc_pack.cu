@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
 
 // SLOPE: d_preact (and out where it is wanted); otherwise out alone, with fewer registers and so more loads under way.
 template <typename T, bool WIDE, bool SLOPE>
-__global__ void __launch_bounds__(kThreads, SLOPE ? 3 : 5)
+__global__ void __launch_bounds__(kThreads, (SLOPE ? 3 : 5) - (sizeof(T) == 4))
     packed_backward_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t rows, int64_t width,
                            int64_t blocks, int act, const T* __restrict__ d_out, int64_t d_out_ld,
                            T* __restrict__ d_preact, int64_t d_preact_ld, T* __restrict__ out, int64_t out_ld)
