@@ -835,19 +835,22 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
   return launched("norm_backward_kernel");
 }
 
+// Three rows ahead where the blocks of an SM have the shared memory for them; of the widest rows two, or none.
 template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
 int launch_backward(cudaStream_t stream, const NormParams& P)
 {
-  if constexpr (WIDE)
+  constexpr size_t have = 200 << 10, widest = (size_t)512 * VPT * 8 * kFetched * sizeof(T); // a round of 512 threads
+  if constexpr (WIDE && 3 * widest <= have)
+    return launch_backward<T, WIDE, TPR, VPT, BIAS, 3>(stream, P);
+  else
   {
-    // Three rows ahead where the blocks of an SM have the shared memory for them, two, or none.
-    const size_t row = (size_t)512 / TPR * kFetched * P.width * sizeof(T), have = 200 << 10;
-    if (row * 3 <= have)
-      return launch_backward<T, true, TPR, VPT, BIAS, 3>(stream, P);
-    if (row * 2 <= have)
-      return launch_backward<T, true, TPR, VPT, BIAS, 2>(stream, P);
+    if constexpr (WIDE)
+    {
+      if ((size_t)512 / TPR * kFetched * P.width * sizeof(T) * 2 <= have)
+        return launch_backward<T, WIDE, TPR, VPT, BIAS, 2>(stream, P);
+    }
+    return launch_backward<T, WIDE, TPR, VPT, BIAS, 0>(stream, P);
   }
-  return launch_backward<T, WIDE, TPR, VPT, BIAS, 0>(stream, P);
 }
 
 template <typename T, bool WIDE>
