@@ -491,7 +491,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
       tc_fence_after();
       if (idle)
       {
-        accumulators_read(lead_tempty + (uint32_t)(acc * 8), lane);
+        if (alive)
+          accumulators_read(lead_tempty + (uint32_t)(acc * 8), lane);
         continue;
       }
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (C::kSets * COLS) + part * C::kShare;
@@ -544,7 +545,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
           for (int i = 0; i < 32; ++i)
             v[i] = __uint_as_float(now[i]);
         }
-        if (c + 1 == C::kShare / 32)
+        if (c + 1 == C::kShare / 32 && alive) // (a warp that gave up hands nothing back: the multiplications end too)
           accumulators_read(lead_tempty + (uint32_t)(acc * 8), lane);
         if (!alive)
         {
