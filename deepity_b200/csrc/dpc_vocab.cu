@@ -22,8 +22,8 @@
 // cores take no wider operand beside bf16 weights, and the sums over it are in 32 bits and are rounded
 // to bf16 themselves.
 //
-// 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low) in the six products
-// whose terms reach 2^-24; s is held in as many planes.  A stage holds the three planes of both operands, so
+// 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low, exactly) in the six products
+// whose terms reach 2^-24 (what is left out is 2^-21 of a product at most, 2^-24 on average); s is held in as many planes.  A stage holds the three planes of both operands, so
 // that six products are made of six loads (a pass over the operands for each product was bound by L2: 4096
 // bytes a step of 256 cycles and SM).  The tensor cores truncate their 32-bit sums, which over the 628
 // additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm); so hi x hi has an accumulator of its
@@ -204,6 +204,32 @@ __device__ __forceinline__ void range_of(const GemmParams& P, int split, int& be
   begin = 0, end = P.kblocks;
   if (P.splits > 1)
     begin = (int)((int64_t)P.kblocks * split / P.splits), end = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
+}
+
+// The three bf16 planes of a float (in the upper halves of words), by truncation: 8 bits each, their sum is the float
+// itself, also where it is above the largest bf16, and they have its sign.  Infinities and NaN are that in every plane, and a
+// plane with nothing left holds the float times 2^-32.  So every plane of a number times an infinity is an infinity of the same
+// sign, and the six products add up to what the definition gives.  (Planes rounded to nearest have zeros and signs of their
+// own, and inf - inf as the second plane of an infinity.  Numbers below 2^-94 have zeros here too: NaN beside an infinity.)
+__device__ __forceinline__ void planes_of(float x, uint32_t (&p)[3])
+{
+  const uint32_t bits = __float_as_uint(x);
+  const float small = x * 2.3283064365386963e-10f; // 2^-32
+  p[0] = bits;
+  float rest = x - __uint_as_float(bits & 0xffff0000u);
+  p[1] = __float_as_uint(rest == 0.0f ? small : rest);
+  rest -= __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+  p[2] = __float_as_uint(rest == 0.0f ? small : rest);
+  if ((bits & 0x7f800000u) == 0x7f800000u)
+    p[0] = p[1] = p[2] = bits & 0x007fffffu ? 0x7fc00000u : bits;
+}
+
+// Words of neighbours in bf16, one of each plane.
+__device__ __forceinline__ void planes_of(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2)
+{
+  uint32_t p[3], q[3];
+  planes_of(a, p), planes_of(b, q);
+  w0 = __byte_perm(p[0], q[0], 0x7632), w1 = __byte_perm(p[1], q[1], 0x7632), w2 = __byte_perm(p[2], q[2], 0x7632);
 }
 
 // 32 logits of a row in units of log 2, -inf outside the vocabulary.
@@ -610,18 +636,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
           {
             __nv_bfloat16* dst = P.slope + row * P.slope_ld + col;
 #pragma unroll
-            for (int pl = 0; pl < C::kPlanes; ++pl, dst += P.slope_plane)
+            for (int i = 0; i < 32; i += 16)
             {
-              float w[16];
+              uint32_t w[C::kPlanes][8];
 #pragma unroll
-              for (int i = 0; i < 32; i += 2)
+              for (int k = 0; k < 8; ++k)
               {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
-                w[i / 2] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
-                v[i] -= __low2float(h), v[i + 1] -= __high2float(h);
+                if constexpr (C::kPlanes == 3)
+                  planes_of(v[i + 2 * k], v[i + 2 * k + 1], w[0][k], w[1][k], w[2][k]);
+                else
+                {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
+                  w[0][k] = *reinterpret_cast<const uint32_t*>(&h);
+                }
               }
-              st8(reinterpret_cast<float*>(dst), w);
-              st8(reinterpret_cast<float*>(dst) + 8, w + 8);
+#pragma unroll
+              for (int pl = 0; pl < C::kPlanes; ++pl)
+                st8(reinterpret_cast<float*>(dst + pl * P.slope_plane + i), reinterpret_cast<const float*>(w[pl]));
             }
           }
         }
@@ -888,12 +919,12 @@ __global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restric
   }
 }
 
-// dst[plane][row][0..ld) = the planes of src[row][0..cols), zeros beyond; rows that do not count are zeros.
+// dst[plane][row][0..ld) = src[row][0..cols) in bf16, or its three planes, zeros beyond; rows that do not count are zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) vocab_planes_kernel(const T* __restrict__ src, int64_t src_ld, int64_t rows,
                                                            int64_t cols, __nv_bfloat16* __restrict__ dst, int64_t ld,
-                                                           int planes, const int64_t* __restrict__ targets,
-                                                           int64_t vocab, int64_t ignore_index)
+                                                           const int64_t* __restrict__ targets, int64_t vocab,
+                                                           int64_t ignore_index)
 {
   const int64_t chunks = ld / 8, total = rows * chunks;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
@@ -904,15 +935,18 @@ __global__ void __launch_bounds__(256) vocab_planes_kernel(const T* __restrict__
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       v[k] = keep && col + k < cols ? to_float(src[row * src_ld + col + k]) : 0.0f;
-    for (int pl = 0; pl < planes; ++pl)
+    __nv_bfloat16* to = dst + row * ld + col;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint4*>(to) = pack8(v); // (the values themselves)
+    else
     {
-      const uint4 h = pack8(v);
-      *reinterpret_cast<uint4*>(dst + ((int64_t)pl * rows + row) * ld + col) = h;
-      float back[8];
-      unpack8(h, back);
+      uint32_t w[3][4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        v[k] -= back[k];
+      for (int k = 0; k < 4; ++k)
+        planes_of(v[2 * k], v[2 * k + 1], w[0][k], w[1][k], w[2][k]);
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl)
+        *reinterpret_cast<uint4*>(to + pl * rows * ld) = make_uint4(w[pl][0], w[pl][1], w[pl][2], w[pl][3]);
     }
   }
 }
@@ -1234,11 +1268,10 @@ int make_planes(cudaStream_t stream, const dpc_vocab_ce* c, const void* src, int
   const int blocks = grid_for(rows * (L.kp / 8));
   if (c->type == DPC_TYPE_F32)
     vocab_planes_kernel<float><<<blocks, 256, 0, stream>>>(static_cast<const float*>(src), src_ld, rows, c->width, to,
-                                                           L.kp, L.planes, targets, c->vocab, c->ignore_index);
+                                                           L.kp, targets, c->vocab, c->ignore_index);
   else
     vocab_planes_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), src_ld, rows,
-                                                                   c->width, to, L.kp, L.planes, targets, c->vocab,
-                                                                   c->ignore_index);
+                                                                   c->width, to, L.kp, targets, c->vocab, c->ignore_index);
   return launched("vocab_planes_kernel");
 }
 

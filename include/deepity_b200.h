@@ -654,7 +654,7 @@ typedef enum dpc_type
  * Backward, from the forward call's lse and g = dL/dloss (grad_loss, grad_stride 1; or one value for all rows,
  * grad_stride 0):  s = g (softmax(l) - onehot);  d_hidden = scale s weight,  d_weight = scale s^T hidden,
  * d_bias = sum of s over the rows.  f32 tensors are multiplied to 32 bits (three bf16 planes each, six
- * products); with bf16 tensors s is rounded to bf16 before its two products.  rows may be 0 (d_weight and
+ * products; an infinity gives the logits that it gives by definition, beside numbers of 2^-94 or more); with bf16 tensors s is rounded to bf16 before its two products.  rows may be 0 (d_weight and
  * d_bias are then zeros); rows, width, vocab and strides 2^28 at most.  A device-side wait that gave up (about 2 s) leaves
  * NaN in the results that were not computed. */
 typedef struct dpc_vocab_ce

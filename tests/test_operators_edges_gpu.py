@@ -1,0 +1,99 @@
+"""Calls of the operators (deepity_b200/operators.py) at the edge of what their documentation allows: infinities, host threads,
+the largest sizes, waits that run out, and how exact 32-bit tensors are."""
+import pytest
+import torch
+
+import operators_common as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def dp(built_library):
+    import deepity_b200
+    return deepity_b200
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, std=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+# ------------------------------------------------------------------------------ infinities in operands
+def infinite_case(rows, kind, seed=0):
+    """The last word's weight holds -inf at column 3, where every row of hidden is positive: its logits are -inf."""
+    g = gen(seed)
+    hidden, weight = normal(g, rows, 40, dtype=kind), normal(g, 301, 40, dtype=kind, std=0.3)
+    hidden[:, 3] = hidden[:, 3].abs() + 0.1
+    weight[300, 3] = -float("inf")
+    return hidden, weight, torch.randint(0, 300, (rows,), generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [2, 5, 8, 9, 40, 300])
+def test_infinite_weight_takes_its_word_out(dp, rows, kind):
+    hidden, weight, targets = infinite_case(rows, TYPES[kind])
+    grad = torch.linspace(0.5, 2.0, rows, device="cuda")
+    want = ref.vocab_reference(hidden, weight[:300], targets, None, 1.0, -100, grad)
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets)
+    ref.check(loss, want["loss"], "loss")
+    ref.check(lse, want["lse"], "lse")
+    got = dp.vocab_cross_entropy_backward(grad, hidden, weight, targets, lse)
+    ref.check(got.weight[:300], want["weight"], "d_weight")
+    assert not got.weight[300].any()
+    keep = torch.arange(40, device="cuda") != 3
+    value, bound = want["hidden"]
+    ref.check(got.hidden[:, keep], (value[:, keep], bound[:, keep]), "d_hidden")
+    assert got.hidden[:, 3].isnan().all()  # 0 * inf
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [2, 5, 40])
+def test_infinite_logits_follow_the_signs(dp, rows, kind):
+    hidden, weight, targets = infinite_case(rows, TYPES[kind], seed=1)
+    clean = dp.vocab_cross_entropy(hidden, weight, targets)
+    moved = hidden.clone()
+    moved[0, 3], moved[1, 3] = -0.5, 0.0  # +inf among the logits; 0 * inf
+    loss, lse = dp.vocab_cross_entropy(moved, weight, targets)
+    assert not loss[:2].isfinite().any() and not lse[:2].isfinite().any()
+    assert torch.equal(loss[2:], clean[0][2:]) and torch.equal(lse[2:], clean[1][2:])
+    targets[0] = 300  # the word that is out: its loss is infinite, the others stay
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets)
+    assert loss[0] == float("inf") and torch.equal(lse, clean[1]) and torch.equal(loss[1:], clean[0][1:])
+    got = dp.vocab_cross_entropy_backward(torch.ones(1, device="cuda"), hidden, weight, targets, lse)
+    assert got.hidden[0, 3].isnan() or got.hidden[0, 3] == float("inf")
+    assert got.weight.isfinite().all()
+
+
+def test_infinite_hidden_stays_in_its_row(dp):
+    hidden, weight, targets = infinite_case(70, torch.float32, seed=2)
+    weight[300, 3] = 0.25
+    clean = dp.vocab_cross_entropy(hidden, weight, targets)
+    hidden[7, 3] = float("inf")  # times weights of both signs
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets)
+    assert not loss[7].isfinite() and not lse[7].isfinite()
+    keep = torch.arange(70, device="cuda") != 7
+    assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(lse[keep], clean[1][keep])
+    weight[:, 3] = -weight[:, 3].abs() - 0.01  # all logits are -inf
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets)
+    assert lse[7] == -float("inf") and loss[7].isnan()
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+def test_numbers_above_the_largest_bf16(dp, rows):
+    """The largest float32 numbers round to an infinity in bf16 and are none themselves."""
+    g = gen(3)
+    hidden, weight = normal(g, rows, 40), normal(g, 300, 40, std=0.3)
+    hidden, weight = hidden * 2.0 ** -10, weight * 2.0 ** 40
+    hidden[:, 3] = 2.0 ** -100
+    weight[:, 3] = torch.linspace(-1.0, 1.0, 300, device="cuda") * torch.finfo(torch.float32).max
+    targets = torch.randint(0, 300, (rows,), generator=g, device="cuda")
+    scale = 2.0 ** -27  # logits up to 2^128 * 2^-100 * 2^-27 = 2
+    want = ref.vocab_reference(hidden, weight, targets, None, scale, -100)
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, scale=scale)
+    ref.check(loss, want["loss"], "loss")
+    ref.check(lse, want["lse"], "lse")
