@@ -986,11 +986,13 @@ __global__ void __launch_bounds__(1024) vocab_gradient_kernel(const float* __res
   }
 }
 
-// out[row][col] = factor * the sum of the splits' sums, in the type of the tensors.
+// out[row][col] = factor * the sum of the splits' sums, in the type of the tensors; 0 in rows that do not count, whose slope of
+// 0 the tensor cores have multiplied with whatever the weights hold (0 times an infinity).
 template <typename T>
 __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict__ sum, int64_t ld, int64_t split_stride,
                                                         int splits, int64_t rows, int64_t cols, T* __restrict__ out,
-                                                        int64_t out_ld, const float* __restrict__ grad_top, float scale)
+                                                        int64_t out_ld, const float* __restrict__ grad_top, float scale,
+                                                        const int64_t* __restrict__ targets, int64_t vocab, int64_t ignore_index)
 {
   const float factor = *grad_top * scale;
   const int64_t chunks = (cols + 3) / 4, total = rows * chunks;
@@ -1003,11 +1005,12 @@ __global__ void __launch_bounds__(256) vocab_sum_kernel(const float* __restrict_
       const float4 w = *reinterpret_cast<const float4*>(sum + s * split_stride + row * ld + col);
       v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
     }
+    const bool keep = counted(targets[row], vocab, ignore_index);
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (col + k < cols)
-        out[row * out_ld + col + k] = from_float<T>(f[k] * factor);
+        out[row * out_ld + col + k] = from_float<T>(keep ? f[k] * factor : 0.0f);
   }
 }
 
@@ -1481,11 +1484,13 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
   const int blocks = grid_for(c->rows * ceil_div(c->width, 4));
   if (c->type == DPC_TYPE_F32)
     vocab_sum_kernel<float><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
-                                                        static_cast<float*>(c->d_hidden), c->d_hidden_stride, grad_top, c->scale);
+                                                        static_cast<float*>(c->d_hidden), c->d_hidden_stride, grad_top, c->scale,
+                                                        c->targets, c->vocab, c->ignore_index);
   else
     vocab_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(sum, L.ks, c->rows * L.ks, L.splits, c->rows, c->width,
                                                                 static_cast<__nv_bfloat16*>(c->d_hidden),
-                                                                c->d_hidden_stride, grad_top, c->scale);
+                                                                c->d_hidden_stride, grad_top, c->scale, c->targets,
+                                                                c->vocab, c->ignore_index);
   return launched("vocab_sum_kernel");
 }
 } // namespace

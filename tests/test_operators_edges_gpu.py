@@ -97,3 +97,15 @@ def test_numbers_above_the_largest_bf16(dp, rows):
     loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, scale=scale)
     ref.check(loss, want["loss"], "loss")
     ref.check(lse, want["lse"], "lse")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_ignored_rows_have_no_gradient_whatever_the_weights_hold(dp, kind):
+    hidden, weight, targets = infinite_case(150, TYPES[kind], seed=4)
+    targets[3], targets[77], targets[149] = -100, 301, -1
+    for bad in (float("inf"), float("nan")):
+        weight[20, 5] = bad
+        loss, lse = dp.vocab_cross_entropy(hidden, weight, targets)
+        got = dp.vocab_cross_entropy_backward(torch.ones(1, device="cuda"), hidden, weight, targets, lse)
+        for row in (3, 77, 149):
+            assert loss[row] == 0 and lse[row] == 0 and not got.hidden[row].any()
