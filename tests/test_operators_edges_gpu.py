@@ -109,3 +109,34 @@ def test_ignored_rows_have_no_gradient_whatever_the_weights_hold(dp, kind):
         got = dp.vocab_cross_entropy_backward(torch.ones(1, device="cuda"), hidden, weight, targets, lse)
         for row in (3, 77, 149):
             assert loss[row] == 0 and lse[row] == 0 and not got.hidden[row].any()
+
+
+# ------------------------------------------------------------------------------ packed activations
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_tanh_is_exact_relative_to_its_value(dp, kind):
+    """Small and large arguments, and both sides of every border between the forms; the kept values' too.
+
+    Errors relative to tanh: a polynomial with 3 roundings, or (1 - e) / (1 + e) with e = exp(-2 |x|) <= 0.37: e is off by 2^-22 of itself
+    and by the rounding of its exponent, 2 |x| log2(e) U < 0.1 * 2^-22 in all, which moves tanh by 1.2 * 0.37 * 2^-22 / 0.46 of
+    itself, a reciprocal is off by 2^-23 and 4 roundings by U each: below 2^-20 together.  The slope 4 e / (1 + e)^2 takes over e's own
+    relative error, 2^-22 + 3 |x| U, two reciprocals and 4 roundings: below 2^-20 + |x| 2^-22; 1 - tanh^2 >= 0.75 loses nothing.
+    For bf16 tensors the border is 1/16: the third term of the series is left out, 2 x^4 / 15 < 2^-18, and above it e's error of
+    2^-22 moves tanh by 0.5 * 2^-22 / 0.062 = 2^-18 of itself: 2^-17."""
+    kind, g = TYPES[kind], gen(5)
+    e = 2.0 ** -20 if kind == torch.float32 else 2.0 ** -17
+    size = 10.0 ** torch.linspace(-30, 1.6, 128 * 128, device="cuda").view(128, 128)
+    border = torch.cat([torch.linspace(at - 0.001, at + 0.001, 128, device="cuda").expand(4, 128) for at in (0.5, 0.0625)])
+    x = torch.cat([size, border, normal(g, 60, 128)])
+    x = torch.cat([x, -x]).to(kind)
+    out, packed = dp.activate_and_pack(x, "tanh")
+    want = x.double().tanh()
+    ref.check(out, (want, (e + ref.half(kind)) * want.abs()), "out")
+    d_x, again = dp.packed_activation_backward(torch.ones_like(x), packed, "tanh", recompute=True)
+    kept = packed.unpack().double()
+    want = kept.tanh()
+    ref.check(again, (want, (e + ref.half(kind)) * want.abs()), "out again")
+    slope = 1.0 / kept.cosh().square()
+    ref.check(d_x, (slope, (e + kept.abs() * 2.0 ** -22 + ref.half(kind)) * slope + 2.0 ** -126), "d_preact")
+    x[0, 0], x[1, 0], x[2, 0] = float("nan"), float("inf"), -float("inf")
+    out = dp.activate_and_pack(x, "tanh")[0]
+    assert out[0, 0].isnan() and out[1, 0] == 1 and out[2, 0] == -1
