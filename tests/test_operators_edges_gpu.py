@@ -140,3 +140,25 @@ def test_tanh_is_exact_relative_to_its_value(dp, kind):
     x[0, 0], x[1, 0], x[2, 0] = float("nan"), float("inf"), -float("inf")
     out = dp.activate_and_pack(x, "tanh")[0]
     assert out[0, 0].isnan() and out[1, 0] == 1 and out[2, 0] == -1
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_esigmoid_is_exact_relative_to_its_value(dp, kind):
+    """0.5 / (1 + |x|) on the left of 0 and 1 less that on the right: the sum, a reciprocal good to 2^-23 and a difference or a square, below
+    2^-21 of the value together."""
+    kind = TYPES[kind]
+    x = 10.0 ** torch.linspace(-6, 30, 64 * 128, device="cuda").view(64, 128)
+    x = torch.cat([x, -x]).to(kind)
+    out, packed = dp.activate_and_pack(x, "esigmoid")
+    half = lambda v: 0.5 / (1 + v.double().abs())  # noqa: E731
+    want = torch.where(x < 0, half(x), 1 - half(x))
+    ref.check(out, (want, (2.0 ** -21 + ref.half(kind)) * want), "out")
+    d_x, again = dp.packed_activation_backward(torch.ones_like(x), packed, "esigmoid", recompute=True)
+    kept = packed.unpack()
+    want = torch.where(kept < 0, half(kept), 1 - half(kept))
+    ref.check(again, (want, (2.0 ** -21 + ref.half(kind)) * want), "out again")
+    slope = 2 * half(kept) ** 2
+    ref.check(d_x, (slope, (2.0 ** -21 + ref.half(kind)) * slope + 2.0 ** -126), "d_preact")
+    x[0, 0], x[1, 0], x[2, 0] = float("nan"), float("inf"), -float("inf")
+    out = dp.activate_and_pack(x, "esigmoid")[0]
+    assert out[0, 0].isnan() and out[1, 0] == 1 and out[2, 0] == 0
