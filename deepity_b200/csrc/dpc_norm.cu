@@ -823,6 +823,8 @@ int launch_forward(cudaStream_t stream, const NormParams& P)
   return launched("norm_forward_kernel");
 }
 
+constexpr size_t kSlotBytes = 200 << 10; // shared memory of an SM for rows that are fetched ahead
+
 template <typename T, bool WIDE, int TPR, int VPT, bool BIAS, int STAGES>
 int launch_backward(cudaStream_t stream, const NormParams& P)
 {
@@ -830,7 +832,12 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
   const unsigned blocks = (unsigned)ceil_div(P.units, Shape<TPR>::kUnits);
   const size_t bytes = (size_t)Shape<TPR>::kUnits * STAGES * kFetched * P.width * sizeof(T);
   if (STAGES > 0)
-    DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  {
+    // The limit belongs to the kernel, not to the launch: with the call's own size, a call on another host thread could
+    // lower it between here and the launch.  The most that any width of this kernel takes is the same for all.
+    constexpr size_t most = std::min(kSlotBytes, (size_t)Shape<TPR>::kThreads * VPT * 8 * STAGES * kFetched * sizeof(T));
+    DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  }
   kernel<<<blocks, Shape<TPR>::kThreads, bytes, stream>>>(P);
   return launched("norm_backward_kernel");
 }
@@ -839,14 +846,14 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
 template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
 int launch_backward(cudaStream_t stream, const NormParams& P)
 {
-  constexpr size_t have = 200 << 10, widest = (size_t)512 * VPT * 8 * kFetched * sizeof(T); // a round of 512 threads
-  if constexpr (WIDE && 3 * widest <= have)
+  constexpr size_t widest = (size_t)512 * VPT * 8 * kFetched * sizeof(T); // a round of 512 threads
+  if constexpr (WIDE && 3 * widest <= kSlotBytes)
     return launch_backward<T, WIDE, TPR, VPT, BIAS, 3>(stream, P);
   else
   {
     if constexpr (WIDE)
     {
-      if ((size_t)512 / TPR * kFetched * P.width * sizeof(T) * 2 <= have)
+      if ((size_t)512 / TPR * kFetched * P.width * sizeof(T) * 2 <= kSlotBytes)
         return launch_backward<T, WIDE, TPR, VPT, BIAS, 2>(stream, P);
     }
     return launch_backward<T, WIDE, TPR, VPT, BIAS, 0>(stream, P);

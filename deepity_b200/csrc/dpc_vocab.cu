@@ -1329,7 +1329,8 @@ int launch_few(cudaStream_t stream, const dpc_vocab_ce* c, int blocks, float2* p
   const bool wide = reinterpret_cast<uintptr_t>(c->weight) % 16 == 0 && c->weight_stride % (16 / sizeof(T)) == 0 &&
                     c->width % 8 == 0;
   auto kernel = wide ? vocab_few_kernel<T, ROWS, true> : vocab_few_kernel<T, ROWS, false>;
-  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  // (the most that a call may take: the limit belongs to the kernel, and calls on other host threads set it too)
+  DPC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewBytes));
   kernel<<<blocks, kFewThreads, bytes, stream>>>(
       static_cast<const T*>(c->hidden), c->hidden_stride, static_cast<const T*>(c->weight), c->weight_stride,
       (int)c->rows, (int)c->width, c->vocab, static_cast<const T*>(c->bias), c->scale * kLog2e, c->targets,

@@ -1,5 +1,7 @@
 """Calls of the operators (deepity_b200/operators.py) at the edge of what their documentation allows: infinities, host threads,
 the largest sizes, waits that run out, and how exact 32-bit tensors are."""
+import threading
+
 import pytest
 import torch
 
@@ -162,3 +164,55 @@ def test_esigmoid_is_exact_relative_to_its_value(dp, kind):
     x[0, 0], x[1, 0], x[2, 0] = float("nan"), float("inf"), -float("inf")
     out = dp.activate_and_pack(x, "esigmoid")[0]
     assert out[0, 0].isnan() and out[1, 0] == 1 and out[2, 0] == 0
+
+
+# ------------------------------------------------------------------------------ host threads
+def at_once(*works):
+    """Every work on a thread and a stream of its own; what they raised."""
+    raised = []
+
+    def call(work):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                work()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 (handed to the test)
+            raised.append(e)
+
+    threads = [threading.Thread(target=call, args=(w,)) for w in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return raised
+
+
+def test_host_threads_with_norms_of_two_widths(dp):
+    """One kernel, whose shared memory goes by the width: neither thread may take it from the other."""
+    def steps(width):
+        def work():
+            g = gen(width)
+            x, w = normal(g, 64, width, dtype=torch.bfloat16), normal(g, width, dtype=torch.bfloat16)
+            _, h, stats = dp.residual_norm(x, pre_weight=w)
+            want = dp.residual_norm_backward(h, None, x, None, stats, pre_weight=w)
+            for _ in range(3000):
+                got = dp.residual_norm_backward(h, None, x, None, stats, pre_weight=w)
+            assert torch.equal(got.stream, want.stream) and torch.equal(got.pre_weight, want.pre_weight)
+        return work
+
+    assert at_once(*(steps(width) for width in (4104, 8192, 4104, 8192))) == []
+
+
+def test_host_threads_with_few_rows_of_two_widths(dp):
+    def steps(width):
+        def work():
+            g = gen(width)
+            hidden, weight = normal(g, 5, width), normal(g, 50, width)
+            targets = torch.arange(5, device="cuda")
+            want = dp.vocab_cross_entropy(hidden, weight, targets)[0]
+            for _ in range(3000):
+                got = dp.vocab_cross_entropy(hidden, weight, targets)[0]
+            assert torch.equal(got, want)
+        return work
+
+    assert at_once(*(steps(width) for width in (256, 2304, 256, 2304))) == []
