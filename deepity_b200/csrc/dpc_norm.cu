@@ -404,7 +404,7 @@ struct Cursor
   {
     if (++row == end)
     {
-      chunk += P.units;
+      chunk = P.chunks - chunk > P.units ? chunk + P.units : P.chunks; // (nothing above their number, which may be 2^31 - 1)
       open(P);
     }
   }

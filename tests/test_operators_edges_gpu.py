@@ -216,3 +216,26 @@ def test_host_threads_with_few_rows_of_two_widths(dp):
         return work
 
     assert at_once(*(steps(width) for width in (256, 2304, 256, 2304))) == []
+
+
+# ------------------------------------------------------------------------------ the largest sizes
+def test_norm_gradient_of_the_most_rows(dp):
+    """2^31 - 1 rows, each a group of its own: the last ones' gradients are those of a call with them alone, and the others' are 0."""
+    torch.cuda.empty_cache()
+    rows, few, g = (1 << 31) - 1, 9, gen(6)
+    big = {k: torch.zeros(rows, 1, device="cuda", dtype=torch.bfloat16) for k in ("new", "branch", "gate", "d_normed")}
+    for t in big.values():
+        t[-few:] = normal(g, few, 1, dtype=torch.bfloat16)
+    stats = torch.zeros(rows, 4, device="cuda")
+    stats[-few:] = normal(g, few, 4)
+    last = {k: t[-few:].clone() for k, t in big.items()}
+
+    def gradients(t, stats):
+        got = dp.residual_norm_backward(t["d_normed"], None, t["new"], t["branch"], stats, gate=t["gate"])
+        return got.stream, got.branch, got.gate
+
+    want = gradients(last, stats[-few:].clone())
+    for a, b in zip(gradients(big, stats), want):
+        assert torch.equal(a[-few:], b) and not a[:-few].any()
+    del big, stats, a
+    torch.cuda.empty_cache()
