@@ -26,7 +26,8 @@ class VocabCe(ctypes.Structure):
                 ("hidden", _p), ("weight", _p), ("bias", _p), ("targets", _p), ("loss", _p), ("lse", _p),
                 ("grad_loss", _p), ("grad_stride", _i64),
                 ("d_hidden", _p), ("d_weight", _p), ("d_hidden_stride", _i64), ("d_weight_stride", _i64),
-                ("d_bias", _p), ("workspace", _p), ("workspace_bytes", _sz)]
+                ("d_bias", _p), ("workspace", _p), ("workspace_bytes", _sz),
+                ("wait_milliseconds", _f), ("wait_bias", _i32)]
 
 
 class ResidualNorm(ctypes.Structure):
@@ -43,7 +44,7 @@ class ResidualNorm(ctypes.Structure):
                 ("d_stream", _p), ("d_branch", _p), ("d_gate", _p),
                 ("d_stream_stride", _i64), ("d_branch_stride", _i64), ("d_gate_stride", _i64),
                 ("d_post_weight", _p), ("d_post_bias", _p), ("d_pre_weight", _p), ("d_pre_bias", _p),
-                ("workspace", _p), ("workspace_bytes", _sz)]
+                ("workspace", _p), ("workspace_bytes", _sz), ("wait_milliseconds", _f), ("wait_bias", _i32)]
 
 
 # name -> (restype, argtypes); every symbol include/deepity_b200.h declares.

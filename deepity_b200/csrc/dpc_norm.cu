@@ -57,6 +57,8 @@ struct NormParams
   int units, chunks, chunks_per_group, rows_per_chunk;
   float *sums, *gate_sums; // [4][units][sums_ld], [chunks][sums_ld]
   int64_t sums_ld;         // the width, up to a multiple of 8
+  long long wait_cycles;   // limit of a wait for a row
+  int keep_back;           // more bytes of a row are waited for than come: the waits run out
 };
 
 // The elements of a row that a thread holds, VPT * 8 of them.  WIDE: vectors of 8 neighbours, 16-byte
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
         for (int s = 0; s < STAGES; ++s)
           dpc::ptx::mbar_init(&filled[u][s], 1);
       give_up[0] = 0;
-      *reinterpret_cast<long long*>(give_up + 2) = dpc::ptx::kWaitCyclesDefault;
+      *reinterpret_cast<long long*>(give_up + 2) = P.wait_cycles;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
@@ -448,7 +450,8 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   if (unit >= P.units)
     return;
   auto fetch = [&](int64_t row, int s) { // by one thread of the unit
-    dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)) + (uint32_t)sizeof(float4));
+    dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)) + (uint32_t)sizeof(float4) +
+                                            (P.keep_back ? 16 : 0));
     auto bulk = [&](uint32_t to, const void* from, uint32_t bytes) {
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
                    "l"(from), "r"(bytes), "r"(dpc::ptx::smem_u32(&full[s]))
@@ -477,14 +480,14 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   float2x dwn[M] = {}, dwp[M] = {}, dg[M] = {}, dbn[BIAS ? M : 1] = {}, dbp[BIAS ? M : 1] = {};
   const bool layer = P.layer != 0;
   bool used = false; // a row before this one has left its slot
+  bool there = true; // no wait has given up: from then on all is NaN, and no slot is filled again
   for (int slot = 0, parity = 0; now.valid(P);)
   {
     const int64_t row = now.row;
     float4 st;
-    bool there = true;
     if constexpr (kAhead)
     {
-      there = dpc::ptx::mbar_wait(&full[slot], parity, give_up);
+      there = there && dpc::ptx::mbar_wait(&full[slot], parity, give_up);
       st = statistics[local][slot];
     }
     else
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
     if (kAhead && t == 0)
     {
       Cursor c = ahead[local];
-      if (used && c.valid(P))
+      if (used && there && c.valid(P))
       {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fetch(c.row, slot == 0 ? STAGES - 1 : slot - 1);
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
     store_pairs<float, WIDE, TPR>(P.sums, at + 2 * plane, width, t, dbn);
     store_pairs<float, WIDE, TPR>(P.sums, at + 3 * plane, width, t, dbp);
   }
-  if (kAhead && give_up[0])
+  if (kAhead && !there)
   {
     // Copies that were not seen to arrive land before the block's shared memory goes away.
     const long long t0 = clock64();
@@ -981,6 +984,9 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
     return dpc::fail(DPC_ERR_INVALID, who + ": " + std::to_string(S.bytes) +
                                           " bytes of workspace on a 256-byte boundary are needed");
   NormParams P = params(c);
+  if (int rc = wait_limit_of(c->wait_milliseconds, &P.wait_cycles))
+    return rc;
+  P.keep_back = c->wait_bias != 0;
   P.dh = c->d_normed, P.dr = c->d_new_stream, P.dx = c->d_stream, P.dy = c->d_branch, P.dg = c->d_gate;
   P.dh_ld = c->d_normed_stride, P.dr_ld = c->d_new_stream_stride, P.dx_ld = c->d_stream_stride;
   P.dy_ld = c->d_branch_stride, P.dg_ld = c->d_gate_stride;

@@ -10,6 +10,7 @@
 #include <string>
 
 #include "dpc_internal.h"
+#include "dpc_tcgen05.cuh"
 
 namespace dpc
 {
@@ -130,6 +131,20 @@ inline EncodeTiledFn encode_fn()
     return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
   }();
   return fn;
+}
+
+// The limit of a call's device-side waits in cycles of the fastest clock, so that it is never shorter than asked.
+inline int wait_limit_of(float milliseconds, long long* cycles)
+{
+  *cycles = ptx::kWaitCyclesDefault;
+  if (milliseconds > 0.0f)
+  {
+    int device = 0, khz = 0;
+    DPC_CUDA(cudaGetDevice(&device));
+    DPC_CUDA(cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, device));
+    *cycles = (long long)((double)milliseconds * khz) + 1;
+  }
+  return DPC_OK;
 }
 
 inline int launched(const char* what)

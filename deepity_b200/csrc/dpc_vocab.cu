@@ -114,6 +114,8 @@ struct GemmParams
   void* out; // EPI_OUT
   int64_t out_ld;
   int out_f32, out_wide;
+  long long wait_cycles; // limit of every wait
+  int keep_back;         // the signals that a tile's sums are complete are not given: the waits for them run out
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -300,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
       mbar_init(&tempty[a], 2 * C::kEpilogueWarps); // both CTAs' epilogue warps arrive on the leader's
     }
     *abort_flag = 0;
-    *reinterpret_cast<volatile long long*>(abort_flag + 2) = kWaitCyclesDefault;
+    *reinterpret_cast<volatile long long*>(abort_flag + 2) = P.wait_cycles;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -366,14 +368,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
             s = 0, phase ^= 1;
         }
       }
-      if (!alive)
-      {
-        // Let copies already in flight land before the CTA's shared memory goes away.
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL * kStages)
-        {
-        }
-      }
     }
   }
   else if (warp == 1)
@@ -435,7 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
             if (++s == kStages)
               s = 0, phase ^= 1;
           }
-          if (alive)
+          if (alive && !P.keep_back)
           {
             tc_commit_pair(smem_u32(&tfull[acc]));
             tc_commit_pair(peer_tfull + (uint32_t)(acc * 8));
@@ -724,6 +718,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
   }
 
   // ------------------------------------------------------------------ teardown
+  // A wait gave up: what is under way (copies into this CTA's shared memory, multiplications that read it) ends before
+  // the pair leaves.  Every wait that does not come true reaches the epilogue warps of both CTAs, whichever warp gave up first, and
+  // the pair leaves together: it is enough that the warps of a CTA that see its flag stay.
+  if (*abort_flag)
+  {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL * kStages)
+    {
+    }
+  }
   __syncwarp();
   tc_fence_before();
   cluster_sync_all(); // neither CTA leaves while the other may still touch its memory
@@ -1141,6 +1145,7 @@ struct Layout
   int64_t ks = 0;    // columns of the sums of d_hidden
   int64_t piece = 0; // vocabulary entries at a time, a multiple of the tile (or all of them)
   int column_parts = 1; // of the rows, in the sums of a bias gradient
+  long long wait_cycles = 0;
   size_t grad_top = 0, columns = 0, hidden = 0, weight = 0, slope = 0, sum = 0, partial = 0, picked = 0, bytes = 0;
 };
 
@@ -1183,6 +1188,8 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   int device = 0, sms = 0;
   DPC_CUDA(cudaGetDevice(&device));
   DPC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  if (int rc = wait_limit_of(c->wait_milliseconds, &L.wait_cycles))
+    return rc;
   L.pairs = std::max(1, sms / 2);
   L.planes = c->type == DPC_TYPE_F32 ? 3 : 1;
   // (backward: the rows that do not count are zeros in the copy, so that an infinity in one of them
@@ -1319,6 +1326,7 @@ GemmParams base_params(const dpc_vocab_ce* c, const Layout& L, int64_t first, ch
   P.bias_f32 = c->type == DPC_TYPE_F32;
   P.targets = c->targets;
   P.vocab = c->vocab, P.first = first, P.ignore_index = c->ignore_index;
+  P.wait_cycles = L.wait_cycles, P.keep_back = c->wait_bias != 0;
   return P;
 }
 

@@ -654,8 +654,9 @@ typedef enum dpc_type
  * Backward, from the forward call's lse and g = dL/dloss (grad_loss, grad_stride 1; or one value for all rows,
  * grad_stride 0):  s = g (softmax(l) - onehot);  d_hidden = scale s weight,  d_weight = scale s^T hidden,
  * d_bias = sum of s over the rows.  f32 tensors are multiplied to 32 bits (three bf16 planes each, six
- * products; an infinity gives the logits that it gives by definition, beside numbers of 2^-94 or more); with bf16 tensors s is rounded to bf16 before its two products.  rows may be 0 (d_weight and
- * d_bias are then zeros); rows, width, vocab and strides 2^28 at most.  A device-side wait that gave up (about 2 s) leaves
+ * products; an infinity gives the logits that it gives by definition, beside numbers of 2^-94 or more); with bf16 tensors s is rounded
+ * to bf16 before its two products.  rows may be 0 (d_weight and
+ * d_bias are then zeros); rows, width, vocab and strides 2^28 at most.  A device-side wait that gave up leaves
  * NaN in the results that were not computed. */
 typedef struct dpc_vocab_ce
 {
@@ -676,6 +677,10 @@ typedef struct dpc_vocab_ce
   void* d_bias; /* or NULL */
   void* workspace;
   size_t workspace_bytes;
+  /* Every wait in the kernels ends after this many milliseconds (0: about 2 s).  wait_bias 1 keeps back a signal that they wait
+   * for, which makes a wait run out; 0 in normal use.  (Up to 2 rows, with f32 up to 8, forward has no waits.) */
+  float wait_milliseconds;
+  int32_t wait_bias;
 } dpc_vocab_ce;
 /* Pointers and strides of the description have to be those of the call: an operand off a 16-byte boundary is copied. */
 DPC_API int dpc_vocab_ce_workspace(const dpc_vocab_ce* call, int backward, size_t* bytes);
@@ -718,6 +723,9 @@ typedef struct dpc_residual_norm
   void *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
   void* workspace;
   size_t workspace_bytes;
+  /* Of backward, as in dpc_vocab_ce: rows that were not seen to arrive, and the sums that they belong to, are NaN. */
+  float wait_milliseconds;
+  int32_t wait_bias;
 } dpc_residual_norm;
 DPC_API int dpc_residual_norm_forward(void* stream, const dpc_residual_norm* call);
 DPC_API int dpc_residual_norm_workspace(const dpc_residual_norm* call, size_t* bytes); /* of backward */

@@ -1,5 +1,6 @@
 """Calls of the operators (deepity_b200/operators.py) at the edge of what their documentation allows: infinities, host threads,
 the largest sizes, waits that run out, and how exact 32-bit tensors are."""
+import ctypes
 import threading
 
 import pytest
@@ -239,3 +240,74 @@ def test_norm_gradient_of_the_most_rows(dp):
         assert torch.equal(a[-few:], b) and not a[:-few].any()
     del big, stats, a
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------ waits that run out
+def entry(name, c, backward=None):
+    """A C entry on torch's current stream, with a workspace of its own."""
+    from deepity_b200 import _lib
+    lib, size, more = _lib.load(), ctypes.c_size_t(), () if backward is None else (backward,)
+    _lib.check(getattr(lib, name + "_workspace")(ctypes.byref(c), *more, ctypes.byref(size)))
+    held = torch.empty(size.value, device="cuda", dtype=torch.uint8)
+    c.workspace, c.workspace_bytes = held.data_ptr(), size.value
+    call = name + ("_forward" if backward == 0 else "_backward")
+    _lib.check(getattr(lib, call)(torch.cuda.current_stream().cuda_stream, ctypes.byref(c)))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kind,rows,width,vocab", [("bf16", 40, 64, 300), ("bf16", 700, 264, 40001), ("f32", 40, 64, 300),
+                                                   ("f32", 300, 1100, 5003)])
+def test_vocab_waits_that_run_out_leave_nan(dp, kind, rows, width, vocab):
+    """A signal is kept back: after 2 ms the kernels give up and return, and what was not computed is NaN.  The next call is right."""
+    from deepity_b200 import _lib
+    g, kind = gen(7), TYPES[kind]
+    hidden, weight, bias = normal(g, rows, width, dtype=kind), normal(g, vocab, width, dtype=kind), normal(g, vocab, dtype=kind)
+    targets = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    targets[5], targets[-1] = -100, vocab
+    counted = (targets >= 0) & (targets < vocab)
+    one = torch.ones(1, device="cuda")
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, bias)
+    want = dp.vocab_cross_entropy_backward(one, hidden, weight, targets, lse, bias)
+    for keep_back in (1, 0):
+        out = {k: torch.full_like(t, 7.0) for k, t in dict(loss=loss, lse=lse, hidden=hidden, weight=weight, bias=bias).items()}
+        c = _lib.VocabCe(rows=rows, width=width, vocab=vocab, hidden_stride=width, weight_stride=width,
+                         type=0 if kind == torch.float32 else 1, scale=1.0, ignore_index=-100, hidden=hidden.data_ptr(),
+                         weight=weight.data_ptr(), bias=bias.data_ptr(), targets=targets.data_ptr(), loss=out["loss"].data_ptr(),
+                         lse=out["lse"].data_ptr(), wait_milliseconds=2.0 * keep_back, wait_bias=keep_back)
+        entry("dpc_vocab_ce", c, 0)
+        c.lse, c.grad_loss, c.grad_stride = lse.data_ptr(), one.data_ptr(), 0
+        c.d_hidden, c.d_hidden_stride, c.d_weight, c.d_weight_stride = out["hidden"].data_ptr(), width, out["weight"].data_ptr(), width
+        c.d_bias = out["bias"].data_ptr()
+        entry("dpc_vocab_ce", c, 1)
+        if keep_back:
+            for name in ("loss", "lse", "hidden"):
+                assert out[name][counted].isnan().all() and not out[name][~counted].any(), name
+            assert out["weight"].isnan().all() and out["bias"].isnan().all()
+        else:
+            assert torch.equal(out["loss"], loss) and torch.equal(out["lse"], lse)
+            assert all(torch.equal(out[name], getattr(want, name)) for name in ("hidden", "weight", "bias"))
+
+
+@pytest.mark.parametrize("kind,rows,width,waits", [("bf16", 3, 256, True), ("bf16", 900, 256, True), ("bf16", 900, 4096, True),
+                                                   ("f32", 900, 2048, True), ("bf16", 9, 12288, True), ("bf16", 9, 16384, False),
+                                                   ("bf16", 9, 255, False)])
+def test_norm_waits_that_run_out_leave_nan(dp, kind, rows, width, waits):
+    """(Two rows ahead of 16384 in bf16 take 4 * 2 * 2 * 16384 bytes, more than an SM's shared memory, and rows off 16 bytes are not
+    fetched ahead: no waits.)"""
+    from deepity_b200 import _lib
+    g, kind = gen(8), TYPES[kind]
+    x, y, d = (normal(g, rows, width, dtype=kind) for _ in range(3))
+    vectors = {k: normal(g, width, dtype=kind) for k in ("gate", "post_weight", "post_bias", "pre_weight", "pre_bias")}
+    new, _, stats = dp.residual_norm(x, y, norm="layer", **vectors)
+    want = dp.residual_norm_backward(d, None, new, y, stats, norm="layer", **vectors)
+    for keep_back in (1, 0):
+        out = {k: torch.full_like(t, 7.0) for k, t in dict(vectors, stream=x, branch=y).items()}
+        c = _lib.ResidualNorm(rows=rows, width=width, groups=1, type=0 if kind == torch.float32 else 1, norm=1, post_norm=1,
+                              stream_scale=1.0, branch_scale=1.0, branch=y.data_ptr(), branch_stride=width, gate_stride=width,
+                              new_stream=new.data_ptr(), new_stream_stride=width, stats=stats.data_ptr(), d_normed=d.data_ptr(),
+                              d_normed_stride=width, d_stream_stride=width, d_branch_stride=width, d_gate_stride=width,
+                              wait_milliseconds=2.0 * keep_back, wait_bias=keep_back,
+                              **{k: v.data_ptr() for k, v in vectors.items()}, **{"d_" + k: v.data_ptr() for k, v in out.items()})
+        entry("dpc_residual_norm", c)
+        for name, t in out.items():
+            assert t.isnan().all() if keep_back and waits else torch.equal(t, getattr(want, name)), name
