@@ -39,9 +39,12 @@ using namespace dpc::ops;
 
 constexpr int64_t kMaxWidth = 16384;
 
+// (Kept at 288 bytes: 16 more took a call of few rows 0.5 us longer.)
 struct NormParams
 {
-  int64_t rows, width;
+  int64_t rows;
+  int width;
+  int wait_kilocycles; // limit of a wait for a row; negative: more bytes are waited for than come, so that the waits run out
   int rows_per_group;
   int layer, post, has_branch;
   float a, b, eps, inv_width;
@@ -57,8 +60,6 @@ struct NormParams
   int units, chunks, chunks_per_group, rows_per_chunk;
   float *sums, *gate_sums; // [4][units][sums_ld], [chunks][sums_ld]
   int64_t sums_ld;         // the width, up to a multiple of 8
-  long long wait_cycles;   // limit of a wait for a row
-  int keep_back;           // more bytes of a row are waited for than come: the waits run out
 };
 
 // The elements of a row that a thread holds, VPT * 8 of them.  WIDE: vectors of 8 neighbours, 16-byte
@@ -173,7 +174,7 @@ __device__ __forceinline__ float2 standardise(float (&v)[N], const NormParams& P
     mean = sum(0.0f, s, false).y * P.inv_width;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      v[i] = column<WIDE, TPR>(t, i) < (int)P.width ? v[i] - mean : 0.0f;
+      v[i] = column<WIDE, TPR>(t, i) < P.width ? v[i] - mean : 0.0f;
   }
   s = 0.0f;
 #pragma unroll
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads) norm_forward_kernel(cons
   constexpr int N = VPT * 8;
   __shared__ float2 buffer[2][TPR / 32];
   RowSum<TPR> sum{buffer};
-  const int t = threadIdx.x & (TPR - 1), width = (int)P.width;
+  const int t = threadIdx.x & (TPR - 1), width = P.width;
   const int64_t row = (int64_t)blockIdx.x * Shape<TPR>::kUnits + threadIdx.x / TPR;
   if (row >= P.rows)
     return; // (a whole warp, where a block has several rows)
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
   __shared__ Cursor ahead[kUnits]; // the next row to fetch: kept by thread 0 of a unit, out of the others' registers
   extern __shared__ __align__(128) uint8_t slots[];
   RowSum<TPR> sum{buffer};
-  const int t = threadIdx.x & (TPR - 1), width = (int)P.width, local = threadIdx.x / TPR;
+  const int t = threadIdx.x & (TPR - 1), width = P.width, local = threadIdx.x / TPR;
   const int unit = blockIdx.x * kUnits + local;
   const uint32_t row_bytes = (uint32_t)(width * sizeof(T));
   const uint32_t slot_at = local * STAGES * kFetched * row_bytes;
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
         for (int s = 0; s < STAGES; ++s)
           dpc::ptx::mbar_init(&filled[u][s], 1);
       give_up[0] = 0;
-      *reinterpret_cast<long long*>(give_up + 2) = P.wait_cycles;
+      *reinterpret_cast<long long*>(give_up + 2) = 1000LL * abs(P.wait_kilocycles);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
     return;
   auto fetch = [&](int64_t row, int s) { // by one thread of the unit
     dpc::ptx::mbar_expect_tx(&full[s], row_bytes * (2 + (P.dr != nullptr) + (P.has_branch != 0)) + (uint32_t)sizeof(float4) +
-                                            (P.keep_back ? 16 : 0));
+                                            (P.wait_kilocycles < 0 ? 16 : 0));
     auto bulk = [&](uint32_t to, const void* from, uint32_t bytes) {
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
                    "l"(from), "r"(bytes), "r"(dpc::ptx::smem_u32(&full[s]))
@@ -805,7 +806,7 @@ bool wide(const dpc_residual_norm* c, std::initializer_list<std::pair<const void
 NormParams params(const dpc_residual_norm* c)
 {
   NormParams P = {};
-  P.rows = c->rows, P.width = c->width;
+  P.rows = c->rows, P.width = (int)c->width;
   P.rows_per_group = (int)std::max<int64_t>(1, c->gate ? c->rows / c->groups : c->rows);
   P.layer = c->norm == DPC_NORM_LAYER, P.post = c->post_norm != 0, P.has_branch = c->branch != nullptr;
   P.a = c->stream_scale, P.b = c->branch_scale, P.eps = c->eps, P.inv_width = 1.0f / (float)c->width;
@@ -984,9 +985,10 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
     return dpc::fail(DPC_ERR_INVALID, who + ": " + std::to_string(S.bytes) +
                                           " bytes of workspace on a 256-byte boundary are needed");
   NormParams P = params(c);
-  if (int rc = wait_limit_of(c->wait_milliseconds, &P.wait_cycles))
+  long long cycles = 0;
+  if (int rc = wait_limit_of(c->wait_milliseconds, &cycles))
     return rc;
-  P.keep_back = c->wait_bias != 0;
+  P.wait_kilocycles = (int)std::min<long long>(cycles / 1000 + 1, 1 << 30) * (c->wait_bias ? -1 : 1);
   P.dh = c->d_normed, P.dr = c->d_new_stream, P.dx = c->d_stream, P.dy = c->d_branch, P.dg = c->d_gate;
   P.dh_ld = c->d_normed_stride, P.dr_ld = c->d_new_stream_stride, P.dx_ld = c->d_stream_stride;
   P.dy_ld = c->d_branch_stride, P.dg_ld = c->d_gate_stride;
