@@ -1230,7 +1230,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   {
     // The contraction of d_hidden, over the piece, is shared out where that fills the GPU's last round of tiles (256
     // tiles on 74 CTA pairs are 4 rounds, in halves 3.5), 4 blocks of it at least each; 3 % a share for its sums.
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(c->rows, kTile) * (L.ks / L.cols));
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(c->rows, kTile) * ceil_div(c->width, L.cols));
     const int64_t blocks = ceil_div(std::min(L.piece, c->vocab), kDepth);
     double best = 0.0;
     for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(L.pairs, blocks / 4)); ++n)

@@ -114,6 +114,26 @@ def test_ignored_rows_have_no_gradient_whatever_the_weights_hold(dp, kind):
             assert loss[row] == 0 and lse[row] == 0 and not got.hidden[row].any()
 
 
+def test_vocab_sums_are_shared_out_by_the_tiles_there_are(dp):
+    """d_hidden's contraction is shared out so that rounds * (1 + 3 % a share) is least, with the tiles that are launched: 128 columns
+    each for float32.  How many shares there are shows in the workspace, where each has its sums."""
+    from deepity_b200 import _lib
+    lib, size = _lib.load(), ctypes.c_size_t()
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    up = lambda v, to: -(-v // to) * to  # noqa: E731
+    for rows, width, vocab in ((777, 515, 10007), (777, 641, 10007), (2048, 1100, 8000), (300, 130, 2000)):
+        c = _lib.VocabCe(rows=rows, width=width, vocab=vocab, hidden_stride=width, weight_stride=width, type=0, scale=1.0,
+                         d_hidden_stride=width, d_weight_stride=width)
+        _lib.check(lib.dpc_vocab_ce_workspace(ctypes.byref(c), 1, ctypes.byref(size)))
+        copies = 6 * up(width, 8)  # three planes of a row
+        rest = 256 + up(rows * copies, 256) + up(vocab * copies, 256) + up(rows * up(vocab, 256) * 6, 256)
+        sums = rows * up(width, 256) * 4
+        shares = (size.value - rest) // sums
+        tiles, blocks = -(-rows // 256) * -(-width // 128), -(-vocab // 64)
+        cost = {n: -(-tiles * n // pairs) / n * (1 + 0.03 * n) for n in range(1, max(1, min(pairs, blocks // 4)) + 1)}
+        assert size.value == rest + up(shares * sums, 256) and cost[shares] == min(cost.values()), (rows, width, shares)
+
+
 # ------------------------------------------------------------------------------ packed activations
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_tanh_is_exact_relative_to_its_value(dp, kind):
