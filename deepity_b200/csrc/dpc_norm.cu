@@ -846,7 +846,8 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
   return launched("norm_backward_kernel");
 }
 
-// Three rows ahead where the blocks of an SM have the shared memory for them; of the widest rows two, or none.
+// Three rows ahead where the blocks of an SM have the shared memory for them; of the widest rows two, or none.  (A kernel's rows
+// are longer than half of what its threads hold, so two of them take `widest` at least.)
 template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
 int launch_backward(cudaStream_t stream, const NormParams& P)
 {
@@ -855,7 +856,7 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
     return launch_backward<T, WIDE, TPR, VPT, BIAS, 3>(stream, P);
   else
   {
-    if constexpr (WIDE)
+    if constexpr (WIDE && widest < kSlotBytes)
     {
       if ((size_t)512 / TPR * kFetched * P.width * sizeof(T) * 2 <= kSlotBytes)
         return launch_backward<T, WIDE, TPR, VPT, BIAS, 2>(stream, P);
