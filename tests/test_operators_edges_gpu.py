@@ -114,6 +114,24 @@ def test_ignored_rows_have_no_gradient_whatever_the_weights_hold(dp, kind):
             assert loss[row] == 0 and lse[row] == 0 and not got.hidden[row].any()
 
 
+@pytest.mark.parametrize("kind,rows,width,vocab", [("f32", 9, 2048, 30000), ("f32", 300, 2048, 50000), ("bf16", 300, 1021, 140001)])
+def test_vocab_forward_in_pieces(dp, kind, rows, width, vocab):
+    """Weights whose copies take more than 256 MB come in pieces: bias, targets and partial sums of the later ones too.  (9 rows: one more
+    than the kernel for few rows takes.)"""
+    kind, g = TYPES[kind], gen(rows)
+    hidden, weight = normal(g, rows, width, dtype=kind), normal(g, vocab, width, dtype=kind, std=2.0 / width ** 0.5)
+    bias = normal(g, vocab, dtype=kind)
+    assert vocab * width * (6 if kind == torch.float32 else 2) > 256 << 20
+    targets = torch.randint(vocab // 2, vocab, (rows,), generator=g, device="cuda")
+    targets[0], targets[1], targets[2] = vocab - 1, 0, -100
+    want = ref.vocab_reference(hidden, weight, targets, bias, 0.5, -100)
+    loss, lse = dp.vocab_cross_entropy(hidden, weight, targets, bias, scale=0.5)
+    ref.check(loss, want["loss"], "loss")
+    ref.check(lse, want["lse"], "lse")
+    # the bounds above are wide; exponentials (2^-22) and logits of |l| <= 10 to 2^-18 (64 truncating additions) leave 4e-5 at most
+    assert (loss.double() - want["loss"][0]).abs().max() < 4e-5 and (lse.double() - want["lse"][0]).abs().max() < 4e-5
+
+
 def test_vocab_sums_are_shared_out_by_the_tiles_there_are(dp):
     """d_hidden's contraction is shared out so that rounds * (1 + 3 % a share) is least, with the tiles that are launched: 128 columns
     each for float32.  How many shares there are shows in the workspace, where each has its sums."""
