@@ -216,6 +216,8 @@ def _norm_call(call, like, branch, norm, post_norm, post_weight, post_bias, gate
         table = call.tensor("gate", gate)
         table = table[None] if table.dim() == 1 else table
         c.groups, gate_width, c.gate_stride = call.matrix("gate", table)
+        if rows == 0 and c.groups == 0:
+            c.groups = 1  # no sequences, each with a gate of its own
         if gate_width != width or c.groups < 1 or rows % c.groups:
             raise ValueError(f"{call.name}: gate is {tuple(gate.shape)}; its last dimension has to be {width}, and "
                              f"its rows have to divide {rows}")

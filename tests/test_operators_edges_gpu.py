@@ -257,7 +257,17 @@ def test_host_threads_with_few_rows_of_two_widths(dp):
     assert at_once(*(steps(width) for width in (256, 2304, 256, 2304))) == []
 
 
-# ------------------------------------------------------------------------------ the largest sizes
+# ------------------------------------------------------------------------------ the smallest and the largest sizes
+def test_norm_of_no_sequences_with_a_gate_each(dp):
+    empty, gate, weight = torch.empty(0, 7, 40, device="cuda"), torch.empty(0, 40, device="cuda"), torch.ones(40, device="cuda")
+    new, normed, stats = dp.residual_norm(empty, empty, gate=gate, pre_weight=weight)
+    got = dp.residual_norm_backward(empty, None, new, empty, stats, gate=gate, pre_weight=weight)
+    assert new.shape == normed.shape == got.stream.shape == (0, 7, 40) and got.gate.shape == (0, 40)
+    assert got.pre_weight.shape == (40,) and not got.pre_weight.any()
+    with pytest.raises(ValueError, match="gate"):
+        dp.residual_norm(torch.ones(2, 40, device="cuda"), torch.ones(2, 40, device="cuda"), gate=gate)
+
+
 def test_norm_gradient_of_the_most_rows(dp):
     """2^31 - 1 rows, each a group of its own: the last ones' gradients are those of a call with them alone, and the others' are 0."""
     torch.cuda.empty_cache()
