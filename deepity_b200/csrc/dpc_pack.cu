@@ -3,7 +3,8 @@
 // A layer's gradient needs f'(x) and, for the weights of the layer after it, f(x): both come from x, so x is all
 // that has to be kept.  Forward writes out = f(x) and x as whole numbers of -127..127 with one 32-bit scale
 // for 128 neighbours of a row (1.03 bytes an element instead of 2 or 4); backward reads them and writes
-// d_preact = d_out f'(x) and, on request, f(x) again.  |x - code * scale| <= max|x| of the block / 254.
+// d_preact = d_out f'(x) and, on request, f(x) again.  |x - code * scale| <= max|x| of the block / 254, but for blocks
+// with nothing of 2^-100 or larger, which are zeros.
 //
 // Bound by memory.  8 threads share a block, 16 elements each, the block's maximum by three shuffles, and nothing is read
 // twice; a thread reads its next part before it works on this one, in 32-byte accesses.  The code is x * (127 / max)
@@ -146,7 +147,7 @@ struct Cells
 };
 
 // gelu(x) = x h, h = 1 / (1 + exp(-2 u)), u = sqrt(2/pi) (x + 0.044715 x^3): the layers' 0.5 x (1 + tanh(u)) with two
-// thirds of its operations; its slope is h + x h (1 - h) (2u)'.  Where exp overflows h is 0; x^2 stops short of
+// thirds of its operations, and other last bits; its slope is h + x h (1 - h) (2u)'.  Where exp overflows h is 0; x^2 stops short of
 // infinity, which times that 0 would be NaN.
 template <bool SLOPE, int N>
 __device__ __forceinline__ void gelu_many(const float (&v)[N], float (&f)[N], float (&d)[N])
@@ -182,7 +183,8 @@ __device__ __forceinline__ void gelu_many(const float (&v)[N], float (&f)[N], fl
 // good from a border on, below which an odd polynomial is taken; the slope is 4 e / (1 + e)^2 or 1 - tanh^2.  32-bit tensors:
 // border 1/2, least squares in x^2 of (tanh(x) / x - 1) / x^2 at Chebyshev nodes (4e-10 off), 2^-20 in all.  bf16, which
 // rounds by 2^-8: border 1/16 and the first two terms of the series (2 x^4 / 15 off), 2^-17 in all, since 16384 x 8192 elements in
-// bf16 wait for instructions (forward 139 us with the layers' form, 166 with the long polynomial, 150 with this one).
+// bf16 wait for instructions (forward 118 us with the layers' form, some 145 with the long polynomial, 133 with this one; float32 183
+// with either).
 template <typename T, bool SLOPE, int N>
 __device__ __forceinline__ void tanh_many(const float (&v)[N], float (&f)[N], float (&d)[N])
 {
@@ -480,7 +482,8 @@ bool wide(int type, const void* p, int64_t stride)
   return !p || (reinterpret_cast<uintptr_t>(p) % 32 == 0 && stride % (type == DPC_TYPE_F32 ? 8 : 16) == 0);
 }
 
-// Blocks of the launch: 8 of 256 threads on every SM, each with a few rounds of work where there is enough.
+// Blocks of the launch: 32 of 256 threads for every SM at most, of which registers let 2 to 5 run at a time; each has a few rounds of
+// work where there is enough.
 template <bool WIDE>
 unsigned grid_for(int64_t blocks)
 {

@@ -6,12 +6,12 @@
 //   s[n,v] = g[n] / G * (exp(l[n,v] - lse[n]) - [v == target[n]])       g = dL/dloss, G = max |g|
 //   d_hidden = scale G s weight      d_weight = scale G s^T hidden      d_bias = G sum_n s
 //
-// Forward: one product whose epilogue keeps, of every 128 columns, the maximum and the sum of the
-// exponentials of a row (8 bytes instead of 128 logits), then a kernel that joins them.  Backward, for
+// Forward: one product whose epilogue keeps, of every 64 columns, the maximum and the sum of the
+// exponentials of a row (8 bytes instead of 64 logits), then a kernel that joins them.  Backward, for
 // a piece of the vocabulary at a time: the product again with an epilogue that writes s, then
-// d_hidden += s weight and d_weight = s^T hidden.  The piece bounds the memory (s of one piece) and the
-// recomputed product is a quarter of the arithmetic; keeping the logits of 8192 rows x 128000 words in 32
-// bits instead would be 4.2 GB.
+// d_hidden += s weight and d_weight = s^T hidden.  The piece bounds the memory for s (256 MB, or 2048 words where they take
+// more: above 65536 rows in bf16) and the recomputed product is a quarter of the arithmetic; keeping the logits of 8192 rows x
+// 128000 words in 32 bits instead would be 4.2 GB (forward's parts of them: 131 MB).
 //
 // One persistent kernel does all four products: 256-row tiles on CTA pairs (cta_group::2), 64-deep
 // stages filled by TMA, accumulators double-buffered in tensor memory so that the epilogue warps work
@@ -26,7 +26,7 @@
 // whose terms reach 2^-24 (what is left out is 2^-21 of a product at most, 2^-24 on average); s is held in as many planes.  A stage holds the three planes of both operands, so
 // that six products are made of six loads (a pass over the operands for each product was bound by L2: 4096
 // bytes a step of 256 cycles and SM).  The tensor cores truncate their 32-bit sums, which over the 628
-// additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm); so hi x hi has an accumulator of its
+// additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm; 7e-7 now); so hi x hi has an accumulator of its
 // own, and a contraction is cut into runs of 8 stages (32 additions) whose sums the epilogue warps add up
 // in registers, rounded to nearest.  They have registers for tiles 128 wide.
 #include <cuda.h>
@@ -744,7 +744,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<COLS, EPI>::kTh
 // memory in 32 bits; a warp multiplies them with kWords words at a time, 8 elements a lane and word, and keeps the
 // maximum and the sum of exponentials of what it has seen.  ROWS: rows, rounded up.  WIDE: 16-byte loads of the weights.
 // 32000 words x 1024, 1 / 2 / 4 / 8 rows: bf16 17 / 19 / 40 / 40 us where the tensor cores take 24, f32 24 / 26 / 31 / 43
-// us where they take 128 (52 of them for the planes): hence up to 2 and up to 8 rows.
+// us where they take 128 (52 of them for the planes): hence up to 2 and up to 8 rows.  With widths of 256 to 4096, 4000 to 128000
+// words and weights off 16 bytes (1021 columns) 3 rows on the tensor cores take 1.1 to 2.5 times as long as 2 here in bf16 (128000 x 256
+// alone: 30 us against 32), 9 rows 1.6 to 3.7 times as long as 8 in f32.
 template <typename T>
 constexpr int kFewRows = sizeof(T) == 2 ? 2 : 8;
 constexpr int kWords = 4, kFewThreads = 256;

@@ -343,7 +343,8 @@ def _packed_backward(call, packed, act, d_out, d_preact, out):
 def activate_and_pack(preact, activation):
     """``(f(preact), packed)``: a layer's activation (a name such as "gelu", or an ``Activation``), with the
     pre-activation [..., width] kept in 8 bits for ``packed_activation_backward``.  Every 128 neighbours of the last dimension share
-    a scale, so an element is off by 1/254 of its block's largest at most; a block with an infinity or a NaN becomes NaN."""
+    a scale, so an element is off by 1/254 of its block's largest at most; a block with nothing of 2^-100 or larger becomes zeros, one with
+    an infinity or a NaN becomes NaN."""
     call = _Call("activate_and_pack", "preact", preact)
     act = _activation(call.name, activation)
     rows, width, stride = call.matrix("preact", preact)

@@ -735,7 +735,8 @@ DPC_API int dpc_residual_norm_backward(void* stream, const dpc_residual_norm* ca
  * scales[row, block] = max|x| / 127, codes[row, col] = round(x * (127 / max|x|)), ties to even; x is then code * scale.  A
  * block with nothing of 2^-100 or larger is held as zeros; one with an infinity or a NaN has a NaN as its scale
  * (and gradient).  codes [rows, width] and scales [rows, ceil(width / 128)] have no gaps; out NULL: not
- * wanted. */
+ * wanted.  The activations are the layers' functions; gelu, tanh and esigmoid are formed another way and differ from the layers' in
+ * their last bits (tanh and esigmoid are exact relative to their value). */
 DPC_API int dpc_activate_and_pack(void* stream, int type, int act, int64_t rows, int64_t width, const void* x,
                                   int64_t x_stride, void* out, int64_t out_stride, int8_t* codes, float* scales);
 /* d_preact = d_out * f'(x) and out = f(x) from the packed x; out NULL: not wanted; d_out and d_preact NULL: only out
