@@ -26,8 +26,7 @@ class VocabCe(ctypes.Structure):
                 ("hidden", _p), ("weight", _p), ("bias", _p), ("targets", _p), ("loss", _p), ("lse", _p),
                 ("grad_loss", _p), ("grad_stride", _i64),
                 ("d_hidden", _p), ("d_weight", _p), ("d_hidden_stride", _i64), ("d_weight_stride", _i64),
-                ("d_bias", _p), ("workspace", _p), ("workspace_bytes", _sz),
-                ("wait_milliseconds", _f), ("wait_bias", _i32)]
+                ("d_bias", _p), ("workspace", _p), ("workspace_bytes", _sz)]
 
 
 class ResidualNorm(ctypes.Structure):
@@ -44,7 +43,7 @@ class ResidualNorm(ctypes.Structure):
                 ("d_stream", _p), ("d_branch", _p), ("d_gate", _p),
                 ("d_stream_stride", _i64), ("d_branch_stride", _i64), ("d_gate_stride", _i64),
                 ("d_post_weight", _p), ("d_post_bias", _p), ("d_pre_weight", _p), ("d_pre_bias", _p),
-                ("workspace", _p), ("workspace_bytes", _sz), ("wait_milliseconds", _f), ("wait_bias", _i32)]
+                ("workspace", _p), ("workspace_bytes", _sz)]
 
 
 # name -> (restype, argtypes); every symbol include/deepity_b200.h declares.
@@ -168,6 +167,7 @@ SIGNATURES = {
     "dpcn_conv_context": (_vp, [_vp]),
     "dpcn_conv_plan": (_vp, [_vp]),
     "dpcn_conv_launch_count": (_i64, [_vp]),
+    "dpc_operators_set_wait_limit": (_i, [ctypes.c_double, _i]),
     "dpc_vocab_ce_workspace": (_i, [ctypes.POINTER(VocabCe), _i, ctypes.POINTER(_sz)]),
     "dpc_vocab_ce_forward": (_i, [_vp, ctypes.POINTER(VocabCe)]),
     "dpc_vocab_ce_backward": (_i, [_vp, ctypes.POINTER(VocabCe)]),

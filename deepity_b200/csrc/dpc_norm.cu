@@ -987,9 +987,9 @@ int backward(cudaStream_t stream, const dpc_residual_norm* c)
                                           " bytes of workspace on a 256-byte boundary are needed");
   NormParams P = params(c);
   long long cycles = 0;
-  if (int rc = wait_limit_of(c->wait_milliseconds, &cycles))
+  if (int rc = wait_limit_now(&cycles))
     return rc;
-  P.wait_kilocycles = (int)std::min<long long>(cycles / 1000 + 1, 1 << 30) * (c->wait_bias ? -1 : 1);
+  P.wait_kilocycles = (int)std::min<long long>(cycles / 1000 + 1, 1 << 30) * (waits.keep_back ? -1 : 1);
   P.dh = c->d_normed, P.dr = c->d_new_stream, P.dx = c->d_stream, P.dy = c->d_branch, P.dg = c->d_gate;
   P.dh_ld = c->d_normed_stride, P.dr_ld = c->d_new_stream_stride, P.dx_ld = c->d_stream_stride;
   P.dy_ld = c->d_branch_stride, P.dg_ld = c->d_gate_stride;

@@ -133,16 +133,24 @@ inline EncodeTiledFn encode_fn()
   return fn;
 }
 
+// What dpc_operators_set_wait_limit said last on this host thread.
+struct Waits
+{
+  double milliseconds = 0.0;
+  bool keep_back = false;
+};
+inline thread_local Waits waits;
+
 // The limit of a call's device-side waits in cycles of the fastest clock, so that it is never shorter than asked.
-inline int wait_limit_of(float milliseconds, long long* cycles)
+inline int wait_limit_now(long long* cycles)
 {
   *cycles = ptx::kWaitCyclesDefault;
-  if (milliseconds > 0.0f)
+  if (waits.milliseconds > 0.0)
   {
     int device = 0, khz = 0;
     DPC_CUDA(cudaGetDevice(&device));
     DPC_CUDA(cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, device));
-    *cycles = (long long)((double)milliseconds * khz) + 1;
+    *cycles = (long long)(waits.milliseconds * khz) + 1;
   }
   return DPC_OK;
 }

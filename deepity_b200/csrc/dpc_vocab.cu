@@ -1190,7 +1190,7 @@ int lay_out(const dpc_vocab_ce* c, bool backward, Layout& L)
   int device = 0, sms = 0;
   DPC_CUDA(cudaGetDevice(&device));
   DPC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-  if (int rc = wait_limit_of(c->wait_milliseconds, &L.wait_cycles))
+  if (int rc = wait_limit_now(&L.wait_cycles))
     return rc;
   L.pairs = std::max(1, sms / 2);
   L.planes = c->type == DPC_TYPE_F32 ? 3 : 1;
@@ -1328,7 +1328,7 @@ GemmParams base_params(const dpc_vocab_ce* c, const Layout& L, int64_t first, ch
   P.bias_f32 = c->type == DPC_TYPE_F32;
   P.targets = c->targets;
   P.vocab = c->vocab, P.first = first, P.ignore_index = c->ignore_index;
-  P.wait_cycles = L.wait_cycles, P.keep_back = c->wait_bias != 0;
+  P.wait_cycles = L.wait_cycles, P.keep_back = waits.keep_back;
   return P;
 }
 
@@ -1505,6 +1505,14 @@ int backward(cudaStream_t stream, const dpc_vocab_ce* c)
   return launched("vocab_sum_kernel");
 }
 } // namespace
+
+int dpc_operators_set_wait_limit(double milliseconds, int wait_bias)
+{
+  if (!(milliseconds <= 60000.0))
+    return dpc::fail(DPC_ERR_INVALID, "dpc_operators_set_wait_limit: a minute at most");
+  waits = {milliseconds, wait_bias != 0};
+  return DPC_OK;
+}
 
 int dpc_vocab_ce_workspace(const dpc_vocab_ce* c, int backward, size_t* bytes)
 {

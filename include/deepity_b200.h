@@ -641,6 +641,12 @@ DPC_API int64_t dpcn_conv_launch_count(dpcn_conv_net* net);
  * inputs nor one another.  Sums, softmax and norm statistics are 32-bit; an output is rounded once.  The same call on the
  * same inputs gives the same bits.
  * ---------------------------------------------------------------------------------- */
+/* Of the calls that the calling host thread makes from now on: every wait in their kernels (for copies of operands and
+ * rows, for accumulators) ends after this many milliseconds (<= 0: about 2 s, the default), and what depends on one that ran out is
+ * NaN.  wait_bias 1 keeps a signal back that the products of the vocabulary loss and the gradients of the residual norms wait
+ * for, which makes their waits run out (the host-side way to exercise the time-out path; 0 in normal use). */
+DPC_API int dpc_operators_set_wait_limit(double milliseconds, int wait_bias);
+
 typedef enum dpc_type
 {
   DPC_TYPE_F32 = 0,
@@ -677,10 +683,6 @@ typedef struct dpc_vocab_ce
   void* d_bias; /* or NULL */
   void* workspace;
   size_t workspace_bytes;
-  /* Every wait in the kernels ends after this many milliseconds (0: about 2 s).  wait_bias 1 keeps back a signal that they wait
-   * for, which makes a wait run out; 0 in normal use.  (Up to 2 rows, with f32 up to 8, forward has no waits.) */
-  float wait_milliseconds;
-  int32_t wait_bias;
 } dpc_vocab_ce;
 /* Pointers and strides of the description have to be those of the call: an operand off a 16-byte boundary is copied. */
 DPC_API int dpc_vocab_ce_workspace(const dpc_vocab_ce* call, int backward, size_t* bytes);
@@ -723,9 +725,6 @@ typedef struct dpc_residual_norm
   void *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
   void* workspace;
   size_t workspace_bytes;
-  /* Of backward, as in dpc_vocab_ce: rows that were not seen to arrive, and the sums that they belong to, are NaN. */
-  float wait_milliseconds;
-  int32_t wait_bias;
 } dpc_residual_norm;
 DPC_API int dpc_residual_norm_forward(void* stream, const dpc_residual_norm* call);
 DPC_API int dpc_residual_norm_workspace(const dpc_residual_norm* call, size_t* bytes); /* of backward */

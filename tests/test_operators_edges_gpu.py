@@ -303,9 +303,21 @@ def entry(name, c, backward=None):
     torch.cuda.synchronize()
 
 
+@pytest.fixture
+def wait_limit(built_library):
+    """wait_limit(1): 2 ms, and a signal is kept back; wait_limit(0): as it was, and so at the test's end."""
+    from deepity_b200 import _lib
+
+    def to(keep_back):
+        _lib.check(_lib.load().dpc_operators_set_wait_limit(2.0 * keep_back, keep_back))
+
+    yield to
+    to(0)
+
+
 @pytest.mark.parametrize("kind,rows,width,vocab", [("bf16", 40, 64, 300), ("bf16", 700, 264, 40001), ("f32", 40, 64, 300),
                                                    ("f32", 300, 1100, 5003)])
-def test_vocab_waits_that_run_out_leave_nan(dp, kind, rows, width, vocab):
+def test_vocab_waits_that_run_out_leave_nan(dp, wait_limit, kind, rows, width, vocab):
     """A signal is kept back: after 2 ms the kernels give up and return, and what was not computed is NaN.  The next call is right."""
     from deepity_b200 import _lib
     g, kind = gen(7), TYPES[kind]
@@ -321,7 +333,8 @@ def test_vocab_waits_that_run_out_leave_nan(dp, kind, rows, width, vocab):
         c = _lib.VocabCe(rows=rows, width=width, vocab=vocab, hidden_stride=width, weight_stride=width,
                          type=0 if kind == torch.float32 else 1, scale=1.0, ignore_index=-100, hidden=hidden.data_ptr(),
                          weight=weight.data_ptr(), bias=bias.data_ptr(), targets=targets.data_ptr(), loss=out["loss"].data_ptr(),
-                         lse=out["lse"].data_ptr(), wait_milliseconds=2.0 * keep_back, wait_bias=keep_back)
+                         lse=out["lse"].data_ptr())
+        wait_limit(keep_back)
         entry("dpc_vocab_ce", c, 0)
         c.lse, c.grad_loss, c.grad_stride = lse.data_ptr(), one.data_ptr(), 0
         c.d_hidden, c.d_hidden_stride, c.d_weight, c.d_weight_stride = out["hidden"].data_ptr(), width, out["weight"].data_ptr(), width
@@ -339,7 +352,7 @@ def test_vocab_waits_that_run_out_leave_nan(dp, kind, rows, width, vocab):
 @pytest.mark.parametrize("kind,rows,width,waits", [("bf16", 3, 256, True), ("bf16", 900, 256, True), ("bf16", 900, 4096, True),
                                                    ("f32", 900, 2048, True), ("bf16", 9, 12288, True), ("bf16", 9, 16384, False),
                                                    ("bf16", 9, 255, False)])
-def test_norm_waits_that_run_out_leave_nan(dp, kind, rows, width, waits):
+def test_norm_waits_that_run_out_leave_nan(dp, wait_limit, kind, rows, width, waits):
     """(Two rows ahead of 16384 in bf16 take 4 * 2 * 2 * 16384 bytes, more than an SM's shared memory, and rows off 16 bytes are not
     fetched ahead: no waits.)"""
     from deepity_b200 import _lib
@@ -354,8 +367,8 @@ def test_norm_waits_that_run_out_leave_nan(dp, kind, rows, width, waits):
                               stream_scale=1.0, branch_scale=1.0, branch=y.data_ptr(), branch_stride=width, gate_stride=width,
                               new_stream=new.data_ptr(), new_stream_stride=width, stats=stats.data_ptr(), d_normed=d.data_ptr(),
                               d_normed_stride=width, d_stream_stride=width, d_branch_stride=width, d_gate_stride=width,
-                              wait_milliseconds=2.0 * keep_back, wait_bias=keep_back,
                               **{k: v.data_ptr() for k, v in vectors.items()}, **{"d_" + k: v.data_ptr() for k, v in out.items()})
+        wait_limit(keep_back)
         entry("dpc_residual_norm", c)
         for name, t in out.items():
             assert t.isnan().all() if keep_back and waits else torch.equal(t, getattr(want, name)), name
