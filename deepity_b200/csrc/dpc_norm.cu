@@ -846,8 +846,8 @@ int launch_backward(cudaStream_t stream, const NormParams& P)
   return launched("norm_backward_kernel");
 }
 
-// Three rows ahead where the blocks of an SM have the shared memory for them; of the widest rows two, or none.  (A kernel's rows
-// are longer than half of what its threads hold, so two of them take `widest` at least.)
+// Three rows ahead where the blocks of an SM have the shared memory for them; of the widest rows two, or none.  (Those rows
+// are longer than half of what their threads hold, so two of them take `widest` at least.)
 template <typename T, bool WIDE, int TPR, int VPT, bool BIAS>
 int launch_backward(cudaStream_t stream, const NormParams& P)
 {

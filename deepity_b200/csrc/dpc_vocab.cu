@@ -23,12 +23,12 @@
 // to bf16 themselves.
 //
 // 32-bit tensors are multiplied as three bf16 planes each (24 bits: hi + mid + low, exactly) in the six products
-// whose terms reach 2^-24 (what is left out is 2^-21 of a product at most, 2^-24 on average); s is held in as many planes.  A stage holds the three planes of both operands, so
-// that six products are made of six loads (a pass over the operands for each product was bound by L2: 4096
-// bytes a step of 256 cycles and SM).  The tensor cores truncate their 32-bit sums, which over the 628
-// additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm; 7e-7 now); so hi x hi has an accumulator of its
-// own, and a contraction is cut into runs of 8 stages (32 additions) whose sums the epilogue warps add up
-// in registers, rounded to nearest.  They have registers for tiles 128 wide.
+// whose terms reach 2^-24 (what is left out is 2^-21 of a product at most, 2^-24 on average); s is held in as many planes.
+// A stage holds the three planes of both operands, so that six products are made of six loads (a pass over the operands
+// for each product was bound by L2: 4096 bytes a step of 256 cycles and SM).  The tensor cores truncate their 32-bit sums,
+// which over the 628 additions of a contraction of 10007 left d_hidden 1.2e-5 off (2-norm; 7e-7 now); so hi x hi has an
+// accumulator of its own, and a contraction is cut into runs of 8 stages (32 additions) whose sums the epilogue warps add
+// up in registers, rounded to nearest.  They have registers for tiles 128 wide.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
